@@ -301,6 +301,115 @@ typedef struct pat_append_args {
 int pat_b200_append_kv(const pat_append_args* args, void* stream);
 
 /* ------------------------------------------------------------------------- *
+ * KV cache held in 4 bits.  No counterpart in the reference, whose caches are 16-bit
+ * (plugin/vllm/attention/backends/prefix_attn.py:828-837).
+ *
+ * Every (token, KV head) row x[head_dim] of K and of V is stored as codes c in 0..15 with a scale and
+ * an offset of its own in the rows' 16-bit type:  lo = min x,  s = round16((max x - lo) / 15),
+ * c = rint((x - lo) / s) clipped to 0..15 (0 where s = 0);  its values are lo + s * c.  A row that
+ * holds a NaN or an infinity is stored as NaN.  The cache is a byte array [num_pages][num_kv_heads]
+ * [page_size / 16][tile], tile = pat_b200_int4_tile_bytes(head_dim) = 16 * head_dim + 128 bytes for the
+ * K and V of 16 tokens of one head (the order inside a tile is described in
+ * pat_b200/csrc/pat_int4.cuh); the tiles of a (page, head) are contiguous, page and head strides are
+ * in bytes, multiples of 16.  head_dim 64 or 128, page_size a multiple of 16, at most 256.
+ * ------------------------------------------------------------------------- */
+size_t pat_b200_int4_tile_bytes(int head_dim);      /* 0 for an unsupported head_dim */
+
+typedef struct pat_int4_rows_args {
+    void* key;                     /* [num_tokens, num_kv_heads, head_dim]; read by the append, written by the gather */
+    void* value;
+    void* cache;
+    const int64_t* slot_mapping;   /* device, [num_tokens]: page * page_size + row */
+    /* strides in elements (multiples of 8), last dimension contiguous, 16-byte aligned bases */
+    int64_t key_token_stride, key_head_stride, value_token_stride, value_head_stride;
+    int64_t page_stride, head_stride;   /* bytes */
+    int64_t num_pages;
+    int32_t num_tokens, num_kv_heads, head_dim, page_size;
+    int32_t dtype;                 /* PAT_DTYPE_* of the rows, and of the scales in the cache */
+    int32_t reserved;
+} pat_int4_rows_args;
+
+/* Quantises the rows of new tokens into their slots.  Slots must be distinct; a negative slot, or one
+ * beyond the cache, is skipped. */
+int pat_b200_append_int4(const pat_int4_rows_args* args, void* stream);
+/* Reads tokens back as 16-bit rows; rows of skipped slots keep what they hold. */
+int pat_b200_gather_int4(const pat_int4_rows_args* args, void* stream);
+
+typedef struct pat_decode_int4_args {
+    const void* q;        /* [batch, q_per_req, num_q_heads, head_dim] */
+    const void* kv_cache; /* 4-bit cache; its scales in the dtype of q */
+    void* out;            /* like q */
+    float* lse_out;       /* optional [batch, q_per_req, num_q_heads] */
+    int64_t q_batch_stride, q_pos_stride, q_head_stride;          /* elements */
+    int64_t out_batch_stride, out_pos_stride, out_head_stride;
+    int64_t page_stride, head_stride;                             /* bytes */
+    int64_t num_pages;
+    int32_t batch, q_per_req, num_q_heads, num_kv_heads, head_dim, page_size;
+    int32_t dtype;        /* PAT_DTYPE_* */
+    int32_t flags;        /* PAT_SKIP_* */
+    float softmax_scale;
+    int32_t wait_limit_us;
+    const int32_t* work_blob;     /* as in pat_decode_args */
+    pat_work_header work;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* status_word;
+} pat_decode_int4_args;
+
+/* pat_b200_decode over a 4-bit cache: same work lists, workspace and status word. */
+int pat_b200_decode_int4(const pat_decode_int4_args* args, void* stream);
+
+/* ------------------------------------------------------------------------- *
+ * Pages of a cache that move: a request that forks copies its part-filled last page, a compaction
+ * moves pages down.  (The reference leaves this to its serving engine.)
+ * Every tensor of the list has the same geometry: page p starts p * page_stride bytes from the
+ * tensor's base and consists of `rows` runs of row_bytes bytes, row_stride bytes apart; all of them
+ * multiples of 16, like the bases.  For every pair (from, to) page `from` is copied over page `to`, in
+ * every tensor.  No page may be the target of two pairs, nor the target of one and the source of
+ * another.
+ * ------------------------------------------------------------------------- */
+typedef struct pat_copy_args {
+    void* const* caches;            /* host array of num_caches device pointers */
+    const int64_t* host_pairs;      /* host, [num_pairs][2], read during the call; a page outside the cache is refused */
+    const int64_t* device_pairs;    /* or device, [num_pairs][2]; pairs with a page outside the cache are skipped */
+    int64_t page_stride, row_stride, row_bytes, num_pages;
+    int32_t num_caches, num_pairs, rows, reserved;
+} pat_copy_args;
+
+int pat_b200_copy_pages(const pat_copy_args* args, void* stream);
+
+/* ------------------------------------------------------------------------- *
+ * Beam selection.  (The reference leaves sampling to its serving engine.)
+ * Of every batch entry the num_out largest of
+ *     scores[b, k] + logits[b, k, v] - log sum_v exp(logits[b, k, v])
+ * over its beams k and tokens v, larger first, ties to the lower k * vocab + v.  A finished beam has
+ * one candidate, pad_token with its score unchanged.  A beam whose score is not finite, or whose
+ * logits hold a NaN or +inf or nothing but -inf, takes no part: its candidates count as -inf, like
+ * masked tokens; they fill the end of the list, lowest index first, where an entry has fewer finite
+ * values than num_out.  num_out <= 128, beams <= 512, beams * ceil(vocab / 8192) <= 8192.
+ * ------------------------------------------------------------------------- */
+enum { PAT_DTYPE_FP32 = 2 };
+
+typedef struct pat_beam_args {
+    const void* logits;             /* [batch, beams, vocab], last dimension contiguous */
+    const float* scores;            /* [batch, beams] */
+    const uint8_t* finished;        /* optional [batch, beams], non-zero = finished */
+    float* out_scores;              /* [batch, num_out], contiguous */
+    int32_t* out_parents;           /* beam each candidate extends */
+    int32_t* out_tokens;
+    int64_t logits_batch_stride, logits_beam_stride;    /* elements */
+    int64_t scores_batch_stride, finished_batch_stride;
+    int32_t batch, beams, vocab, num_out;
+    int32_t dtype;                  /* PAT_DTYPE_FP16 / BF16 / FP32 */
+    int32_t pad_token;
+    void* workspace;                /* scratch of the call, 16-byte aligned; nothing in it has to hold a value */
+    size_t workspace_bytes;
+} pat_beam_args;
+
+size_t pat_b200_beam_workspace_bytes(int batch, int beams, int vocab, int num_out);    /* 0: sizes out of range */
+int pat_b200_beam_select(const pat_beam_args* args, void* stream);
+
+/* ------------------------------------------------------------------------- *
  * KV-head sharding: head order after the optional all-gather of the outputs.
  * The reference has no multi-GPU path of its own (a tensor-parallel vLLM hands its backend
  * per-rank head counts, plugin/vllm/attention/backends/prefix_attn.py:617-618, and never gathers).

@@ -14,6 +14,10 @@ from .async_tree import AsyncTree
 # a kernel whose bounded wait ran out
 from ._prefix_attn import check_status, status_word
 from .planner import DecodePlanner
+# nor are the operators of a beam search over a cache held in 4 bits (see also cache_ops)
+from ._prefix_attn import prefix_attn_with_int4_kvcache
+from .beam import PagePool, beam_select
+from .planner import BeamPlanner
 
 __all__ = [
     "prefix_attn_with_kvcache",

@@ -70,6 +70,21 @@ def set_default_config(cfg: Optional[WorkConfig]) -> None:
     _default_config = cfg
 
 
+def int4_config() -> WorkConfig:
+    """Options of the work lists for a 4-bit cache."""
+    cfg = WorkConfig(**{n: getattr(default_config(), n) for n in WorkConfig.__slots__})
+    cfg.disable_dense = 1
+    return cfg
+
+
+def _config_of(kv_cache_dtype: str) -> WorkConfig:
+    if kv_cache_dtype == "int4":
+        return int4_config()
+    if kv_cache_dtype not in ("auto", "float16", "bfloat16"):
+        raise RuntimeError(f"kv_cache_dtype {kv_cache_dtype!r} is not supported (16-bit or int4 caches only)")
+    return default_config()
+
+
 _WS_HEAD = 256      # bytes of control words at the head of a workspace (include/pat_b200.h)
 
 
@@ -313,7 +328,9 @@ class KernelInfo:
             v[name] = [move(t) for t in v[name]]
         v["num_split_per_seq"] = move(v["num_split_per_seq"])
 
-    def to_gpu(self, device: Union[torch.device, str]) -> None:
+    def to_gpu(self, device: Union[torch.device, str], kv_cache_dtype: str = "auto") -> None:
+        """``kv_cache_dtype="int4"``: the plan is for ``prefix_attn_with_int4_kvcache``."""
+        cfg = _config_of(kv_cache_dtype)
         device = torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
@@ -321,7 +338,7 @@ class KernelInfo:
         if self._vals is not None:
             self._move(self._vals, device)
         if device.type == "cuda":
-            self.device_work(device)
+            self.device_work(device, cfg)
             check_status(device, synchronize=False)     # a failed wait of an earlier step surfaces here
 
     def device_work(self, device: torch.device, cfg: Optional[WorkConfig] = None, q_per_req: int = 1) -> DeviceWork:
@@ -818,6 +835,112 @@ def prefix_attn_with_kvcache(*args, **kwargs) -> None:
 
     with torch.cuda.device(q.device):
         _run(q, k_cache, v_cache, work, scale, out, lse_out, status, flags, wait_limit_us)
+
+
+def _strides(t: torch.Tensor):
+    """Strides with those of one-element dimensions, which nobody uses and torch leaves arbitrary, set to
+    the dense ones."""
+    out, dense = list(t.stride()), 1
+    for i in reversed(range(t.dim())):
+        if t.shape[i] <= 1:
+            out[i] = dense
+        dense = max(dense, out[i] * t.shape[i])
+    return out
+
+
+def _run_int4(q, kv_cache, work: DeviceWork, scale: float, out, lse_out, status, flags, wait_limit_us):
+    lib = N.load()
+    stream = torch.cuda.current_stream(q.device)
+    work.order_after_upload(stream)
+    if status is None:
+        status = status_word(q.device)
+    key = (q.data_ptr(), kv_cache.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse_out is not None else 0,
+           status.data_ptr(), stream.cuda_stream, q.shape, q.stride(), kv_cache.shape, kv_cache.stride(), out.stride(),
+           q.dtype, float(scale), int(flags), int(wait_limit_us))
+    cached = work._args
+    if cached is not None and cached[0] == key:
+        a = cached[1]
+    else:
+        B, T, H, D = q.shape
+        a = N.DecodeInt4Args()
+        a.q, a.kv_cache, a.out = q.data_ptr(), kv_cache.data_ptr(), out.data_ptr()
+        a.lse_out = lse_out.data_ptr() if lse_out is not None else None
+        a.q_batch_stride, a.q_pos_stride, a.q_head_stride = _strides(q)[:3]
+        a.out_batch_stride, a.out_pos_stride, a.out_head_stride = _strides(out)[:3]
+        a.page_stride, a.head_stride = _strides(kv_cache)[:2]
+        a.num_pages = kv_cache.shape[0]
+        a.batch, a.q_per_req, a.num_q_heads, a.num_kv_heads, a.head_dim = B, T, H, kv_cache.shape[1], D
+        a.page_size = kv_cache.shape[2] * 16
+        a.dtype = _DTYPES[q.dtype]
+        a.flags = int(flags)
+        a.softmax_scale = float(scale)
+        a.wait_limit_us = int(wait_limit_us)
+        a.work_blob = work.blob.data_ptr()
+        a.work = work.header
+        need = lib.pat_b200_workspace_bytes(C.byref(work.header), H, D)
+        ws = work.workspace(need, stream, q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        a.status_word = status.data_ptr()
+        work._args = (key, a)
+    rc = lib.pat_b200_decode_int4(C.byref(a), C.c_void_p(stream.cuda_stream))
+    if rc != 0:
+        raise RuntimeError(f"prefix_attn_with_int4_kvcache failed: {N.strerror(rc)} ({rc})")
+
+
+def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree, softmax_scale: float,
+                                  out: torch.Tensor, lse_out: Optional[torch.Tensor] = None, *, _status=None,
+                                  _flags: int = 0, _wait_limit_us: int = 0) -> None:
+    """``prefix_attn_with_kvcache`` (tree form) over a KV cache held in 4 bits; writes ``out`` in place.
+
+    ``kv_cache``: uint8 ``[pages, kv_heads, page_size / 16, tile bytes]`` as ``cache_ops.int4_cache_shape``
+    gives it, filled by ``cache_ops.reshape_and_cache_int4`` with rows of ``q``'s dtype; page and head strides are
+    free.  ``tree``: a ``PrefixTreeCPP`` (or an ``AsyncTree`` holding one) whose plan was sent with
+    ``kernel_info.to_gpu(device, kv_cache_dtype="int4")``.  ``q``, ``out``, ``softmax_scale`` and ``lse_out`` are
+    those of ``prefix_attn_with_kvcache``, several query tokens per request included.  A request (or
+    position) that sees no token gets zeros, and -inf in ``lse_out``.
+
+    The products run on the exact codes; scales, offsets, softmax and sums are fp32, and the
+    probabilities are rounded to ``q``'s dtype for the second product as in the 16-bit op."""
+    _check(q.dtype in _DTYPES, "only support fp16 and bf16 data type")
+    for t, n in ((q, "q"), (kv_cache, "kv_cache"), (out, "out")):
+        _check(t.is_cuda, f"{n} must be on CUDA")
+        _check(t.device == q.device, f"{n} must be on the device of q")
+    _check(q.dim() == 4, "q must have shape (batch_size, seqlen_q, n_heads, head_size)")
+    B, T, H, D = q.shape
+    _check(D in (64, 128), "head_size_og must be 64 / 128 currently")
+    _check(kv_cache.dtype == torch.uint8 and kv_cache.dim() == 4, "kv_cache must be uint8 [pages, kv_heads, page_size / 16, tile bytes]")
+    tile = int(N.load().pat_b200_int4_tile_bytes(D))
+    Hkv, page = kv_cache.shape[1], kv_cache.shape[2] * 16
+    _check(kv_cache.shape[3] == tile and kv_cache.stride(3) == 1 and (page == 16 or kv_cache.stride(2) == tile),
+           "kv_cache was laid out for another head_size, or its tiles are not contiguous")
+    _check(0 < page <= 256, "Paged KV cache block size must be between 16 and 256")
+    _check(Hkv > 0 and H % Hkv == 0, "Number of heads in key/value must divide number of heads in query")
+    ratio = H // Hkv
+    _check(ratio in (1, 2, 4, 8), "only support QGA with hq/hkv = 1, 2, 4, 8 now.")
+    _check(B > 0, "batch size must be positive")
+    _check(1 <= T <= 64, "seqlen_q must be between 1 and 64")
+    _check(out.dtype == q.dtype and tuple(out.shape) == tuple(q.shape), "out must be a CUDA tensor with the shape and dtype of q")
+    for t, n in ((q, "q"), (out, "out")):
+        _check(t.stride(-1) == 1, "Input tensor must have contiguous last dimension")
+        _check(all(s > 0 and s % 8 == 0 for s in _strides(t)[:3]) and t.data_ptr() % 16 == 0,
+               f"{n} rows must be 16-byte aligned and not overlap")
+    if lse_out is not None:
+        _check(lse_out.is_cuda and lse_out.device == q.device and lse_out.dtype == torch.float32 and lse_out.is_contiguous()
+               and tuple(lse_out.shape) == ((B, H) if T == 1 else (B, T, H)),
+               "lse_out must be a contiguous float32 CUDA tensor [batch, heads] ([batch, seqlen_q, heads])")
+    inner = getattr(tree, "tree", None)         # an AsyncTree hands over its built tree
+    if not isinstance(tree, PrefixTreeCPP) and isinstance(inner, PrefixTreeCPP):
+        tree = inner
+    _check(isinstance(tree, PrefixTreeCPP), "tree must be a PrefixTreeCPP")
+    info = tree.kernel_info
+    _check(info._device is not None and info._device.type == "cuda", "the plan was not sent to the GPU (kernel_info.to_gpu)")
+    _check(tree._batch() == B, f"the plan was built for {tree._batch()} requests, q has {B}")
+    _check(tree._hratio == ratio, "the plan was packed for a different HRatio than q / kv_cache imply")
+    _check(tree._kv_heads == Hkv, "the plan was packed for a different number of KV heads than kv_cache has")
+    _check(tree.block_size == page, "the plan was built for a different page size than kv_cache has")
+    work = info.device_work(q.device, int4_config(), T)
+    with torch.cuda.device(q.device):
+        _run_int4(q, kv_cache, work, softmax_scale, out, lse_out, _status, _flags, _wait_limit_us)
 
 
 def last_launch_count() -> int:

@@ -18,7 +18,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libpat_b200.so")
-SOURCES = ["pat_tree.cpp", "pat_work.cpp", "pat_capi.cpp", "pat_decode.cu", "pat_append.cu", "pat_gather.cu"]
+SOURCES = ["pat_tree.cpp", "pat_work.cpp", "pat_capi.cpp", "pat_decode.cu", "pat_append.cu", "pat_gather.cu",
+           "pat_int4.cu", "pat_pages.cu", "pat_beam.cu"]
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))) + [
     os.path.join("..", "..", "include", "pat_b200.h")]
 

@@ -1,4 +1,5 @@
-"""KV-cache append, the step right before decode attention in a serving loop.
+"""Cache operations around decode attention in a serving loop: the KV-cache append right before it, the
+same for a cache held in 4 bits, and copies of whole pages (a request that forks, a compaction).
 
 ``reshape_and_cache_flash`` has the signature of vLLM's op of the same name, which the
 reference's serving backend calls through ``torch.ops._C_cache_ops``
@@ -8,8 +9,9 @@ PyTorch's current stream; there is no fallback.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from typing import Optional, Sequence, Union
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -67,3 +69,178 @@ def reshape_and_cache_flash(key: torch.Tensor, value: torch.Tensor, key_cache: t
         rc = N.load().pat_b200_append_kv(C.byref(a), C.c_void_p(stream))
     if rc != 0:
         raise RuntimeError(f"reshape_and_cache_flash failed: {N.strerror(rc)} ({rc})")
+
+
+# --------------------------------------------------------------------------- cache held in 4 bits
+def int4_tile_bytes(head_dim: int) -> int:
+    """Bytes of K and V of 16 tokens of one KV head in a 4-bit cache."""
+    n = int(N.load().pat_b200_int4_tile_bytes(int(head_dim)))
+    if n == 0:
+        raise RuntimeError("head_dim must be 64 / 128 currently")
+    return n
+
+
+def int4_cache_shape(num_pages: int, page_size: int, kv_heads: int, head_dim: int):
+    """Shape of the uint8 tensor that holds ``num_pages`` pages of K and V in 4 bits.
+
+    Every (token, KV head) row of K and of V is stored as codes ``c`` in 0..15 with a scale and an
+    offset of its own in the model's 16-bit type: ``lo = min x``, ``s = round16((max x - lo) / 15)``,
+    ``c = rint((x - lo) / s)``; its values are ``lo + s * c``.  That is ``head_dim + 8`` bytes per token
+    and KV head instead of ``4 * head_dim``.  Allocate it zeroed or not: only slots that were written are
+    ever read."""
+    if page_size < 16 or page_size % 16 != 0 or page_size > 256:
+        raise RuntimeError("page_size must be a multiple of 16, at most 256")
+    return (int(num_pages), int(kv_heads), int(page_size) // 16, int4_tile_bytes(head_dim))
+
+
+def _check_int4_cache(kv_cache: torch.Tensor, heads: int, dim: int) -> None:
+    if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 4:
+        raise RuntimeError("kv_cache must be uint8 [pages, kv_heads, page_size / 16, tile bytes]")
+    tile = int4_tile_bytes(dim)
+    if kv_cache.shape[1] != heads or kv_cache.shape[3] != tile:
+        raise RuntimeError("kv_cache disagrees with the rows on kv_heads / head_dim")
+    if kv_cache.stride(3) != 1 or (kv_cache.shape[2] > 1 and kv_cache.stride(2) != tile):
+        raise RuntimeError("the tiles of a page and head must be contiguous in kv_cache")
+
+
+def _int4_rows(name: str, fn: str, key, value, kv_cache, slot_mapping) -> None:
+    for n, t in (("key", key), ("value", value), ("kv_cache", kv_cache), ("slot_mapping", slot_mapping)):
+        if not t.is_cuda:
+            raise RuntimeError(f"{n} must be a CUDA tensor")
+        if t.device != key.device:
+            raise RuntimeError(f"{n} must be on the device of key")
+    if key.dtype not in _DTYPES or value.dtype != key.dtype:
+        raise RuntimeError("key and value must share one dtype, fp16 or bf16")
+    if key.dim() != 3 or value.shape != key.shape:
+        raise RuntimeError("key and value must be [num_tokens, kv_heads, head_dim]")
+    tokens, heads, dim = key.shape
+    _check_int4_cache(kv_cache, heads, dim)
+    for n, t in (("key", key), ("value", value)):
+        if t.stride(-1) != 1:
+            raise RuntimeError(f"{n} must have a contiguous last dimension")
+    slots = slot_mapping.flatten()
+    if slots.dtype != torch.int64:
+        slots = slots.to(torch.int64)
+    slots = slots.contiguous()
+    if slots.numel() < tokens:
+        raise RuntimeError("slot_mapping is shorter than the number of tokens")
+    if kv_cache.shape[0] == 0 or tokens == 0 or heads == 0:
+        return
+    a = N.Int4RowsArgs()
+    a.key, a.value, a.cache, a.slot_mapping = key.data_ptr(), value.data_ptr(), kv_cache.data_ptr(), slots.data_ptr()
+    # (a dimension of one element has a stride nobody uses, and torch may report any)
+    a.key_token_stride, a.value_token_stride = (t.stride(0) if tokens > 1 else heads * dim for t in (key, value))
+    a.key_head_stride, a.value_head_stride = (t.stride(1) if heads > 1 else dim for t in (key, value))
+    a.page_stride = kv_cache.stride(0) if kv_cache.shape[0] > 1 else kv_cache[0].numel()
+    a.head_stride = kv_cache.stride(1) if heads > 1 else kv_cache.shape[2] * kv_cache.shape[3]
+    a.num_pages = kv_cache.shape[0]
+    a.num_tokens, a.num_kv_heads, a.head_dim, a.page_size = tokens, heads, dim, kv_cache.shape[2] * 16
+    a.dtype = _DTYPES[key.dtype]
+    with torch.cuda.device(key.device):
+        stream = torch.cuda.current_stream().cuda_stream
+        rc = getattr(N.load(), fn)(C.byref(a), C.c_void_p(stream))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed: {N.strerror(rc)} ({rc})")
+
+
+def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
+                           slot_mapping: torch.Tensor) -> None:
+    """Quantises ``key[i]`` / ``value[i]`` (``[num_tokens, kv_heads, head_dim]``, fp16 or bf16) into the 4-bit
+    cache (``int4_cache_shape``) at ``slot_mapping[i] = page * page_size + row``.  Tokens with a
+    negative slot, or one beyond the cache, are skipped; slots must be distinct.  A row that holds a NaN or an
+    infinity is stored as NaN.  All rows of a cache have one dtype (its scales are stored in it)."""
+    _int4_rows("reshape_and_cache_int4", "pat_b200_append_int4", key, value, kv_cache, slot_mapping)
+
+
+def gather_cache_int4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> None:
+    """Reads the tokens at ``slot_mapping`` back from a 4-bit cache into ``key`` / ``value``
+    (``[num_tokens, kv_heads, head_dim]``, the dtype that was appended), e.g. a cached prefix for a
+    prefill that runs on 16-bit keys.  Rows of skipped slots (see ``reshape_and_cache_int4``) keep what they hold."""
+    _int4_rows("gather_cache_int4", "pat_b200_gather_int4", key, value, kv_cache, slot_mapping)
+
+
+# --------------------------------------------------------------------------- moving pages
+def _page_geometry(cache: torch.Tensor):
+    """(rows, row_stride, row_bytes) of one page of ``cache``: runs of contiguous bytes at one stride."""
+    item = cache.element_size()
+    run, rows, row_stride = item, 1, 0
+    for size, stride in zip(reversed(cache.shape[1:]), reversed(cache.stride()[1:])):
+        if size == 1:
+            continue
+        stride *= item
+        if rows == 1 and stride == run:
+            run *= size
+        elif rows == 1:
+            rows, row_stride = size, stride
+        elif stride == rows * row_stride:
+            rows *= size
+        else:
+            return None
+    return rows, row_stride or run, run
+
+
+def copy_pages(caches: Union[torch.Tensor, Sequence[torch.Tensor]], mapping) -> None:
+    """Copies page ``from`` over page ``to`` in every tensor of ``caches``, for every pair ``(from, to)`` of
+    ``mapping``.
+
+    ``caches``: paged caches of any kind (K and V of all layers, 16-bit or 4-bit), all of one shape,
+    dtype and strides; dimension 0 counts pages.  ``mapping``: ``[n, 2]``, a list or an integer CPU tensor
+    (what ``PagePool.fork`` and ``PagePool.compact`` return; checked: pages inside the cache, and no page that is the target
+    of one pair may occur in another), or an int64 CUDA tensor with the same contract, which is not
+    checked; pairs with a page outside the cache are then skipped.  A host mapping travels in the
+    launch itself: a CUDA graph captured around the call repeats that mapping."""
+    caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
+    on_device = isinstance(mapping, torch.Tensor) and mapping.is_cuda
+    if not on_device:
+        mapping = torch.as_tensor(mapping, dtype=torch.int64).contiguous()
+        if mapping.numel() == 0:
+            mapping = mapping.reshape(0, 2)
+    if mapping.dim() != 2 or mapping.shape[1] != 2:
+        raise RuntimeError("mapping must be [n, 2]: pairs (from, to)")
+    if on_device and (mapping.dtype != torch.int64 or not mapping.is_contiguous()):
+        raise RuntimeError("a CUDA mapping must be contiguous int64")
+    if not caches:
+        return
+    first = caches[0]
+    for t in caches:
+        if not t.is_cuda:
+            raise RuntimeError("caches must be CUDA tensors")
+        if t.device != first.device or t.dtype != first.dtype or t.shape != first.shape or t.stride() != first.stride():
+            raise RuntimeError("caches must share device, dtype, shape and strides")
+    if on_device and mapping.device != first.device:
+        raise RuntimeError("mapping must be on the device of the caches, or on the host")
+    if first.dim() < 2:
+        raise RuntimeError("caches must be [pages, ...]")
+    pages = first.shape[0]
+    n = mapping.shape[0]
+    if not on_device and n:
+        src, dst = mapping[:, 0], mapping[:, 1]
+        if int(mapping.min()) < 0 or int(mapping.max()) >= pages:
+            raise RuntimeError(f"mapping names a page outside the cache ({pages} pages)")
+        flat = dst.numpy()
+        hit = np.zeros(pages, dtype=np.int32)
+        np.add.at(hit, flat, 1)
+        if hit.max() > 1:
+            raise RuntimeError("a page is the target of two pairs")
+        if hit[src.numpy()].any():
+            raise RuntimeError("a page is both a source and a target")
+    if n == 0 or first.numel() == 0:
+        return
+    geometry = _page_geometry(first)
+    if geometry is None:
+        raise RuntimeError("a page must consist of equally long contiguous runs at one stride")
+    a = N.CopyArgs()
+    ptrs = (C.c_void_p * len(caches))(*[t.data_ptr() for t in caches])
+    a.caches = C.cast(ptrs, C.c_void_p)
+    if on_device:
+        a.device_pairs = mapping.data_ptr()
+    else:
+        a.host_pairs = mapping.data_ptr()
+    a.rows, a.row_stride, a.row_bytes = geometry
+    a.page_stride = first.stride(0) * first.element_size() if pages > 1 else a.rows * a.row_stride
+    a.num_pages, a.num_caches, a.num_pairs = pages, len(caches), n
+    with torch.cuda.device(first.device):
+        stream = torch.cuda.current_stream().cuda_stream
+        rc = N.load().pat_b200_copy_pages(C.byref(a), C.c_void_p(stream))
+    if rc != 0:
+        raise RuntimeError(f"copy_pages failed: {N.strerror(rc)} ({rc})")

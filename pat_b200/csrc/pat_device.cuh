@@ -54,7 +54,7 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 constexpr uint64_t kDefaultWaitNs = 1000ull * 1000ull * 1000ull;
 // The polling loop is kept out of line: a kernel waits in many places, and warps that run a
 // little code per tile (TMA producers, the MMA issuer) are bound by instruction fetch.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
     const uint64_t start = global_timer_ns();
     for (uint32_t i = 1; i < kMaxPolls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
