@@ -340,6 +340,10 @@ typedef struct pat_decode_int4_args {
     const void* kv_cache; /* 4-bit cache; its scales in the dtype of q */
     void* out;            /* like q */
     float* lse_out;       /* optional [batch, q_per_req, num_q_heads] */
+    const int32_t* work_blob;     /* as in pat_decode_args */
+    void* workspace;
+    int32_t* status_word;
+    size_t workspace_bytes;
     int64_t q_batch_stride, q_pos_stride, q_head_stride;          /* elements */
     int64_t out_batch_stride, out_pos_stride, out_head_stride;
     int64_t page_stride, head_stride;                             /* bytes */
@@ -349,11 +353,7 @@ typedef struct pat_decode_int4_args {
     int32_t flags;        /* PAT_SKIP_* */
     float softmax_scale;
     int32_t wait_limit_us;
-    const int32_t* work_blob;     /* as in pat_decode_args */
     pat_work_header work;
-    void* workspace;
-    size_t workspace_bytes;
-    int32_t* status_word;
 } pat_decode_int4_args;
 
 /* pat_b200_decode over a 4-bit cache: same work lists, workspace and status word. */
@@ -370,10 +370,11 @@ int pat_b200_decode_int4(const pat_decode_int4_args* args, void* stream);
  * ------------------------------------------------------------------------- */
 typedef struct pat_copy_args {
     void* const* caches;            /* host array of num_caches device pointers */
-    const int64_t* host_pairs;      /* host, [num_pairs][2], read during the call; a page outside the cache is refused */
+    const int64_t* host_pairs;      /* host, [num_pairs][2], read during the call; a mapping that breaks the rules is
+                                       refused with PAT_ERR_BAD_PLAN */
     const int64_t* device_pairs;    /* or device, [num_pairs][2]; pairs with a page outside the cache are skipped */
     int64_t page_stride, row_stride, row_bytes, num_pages;
-    int32_t num_caches, num_pairs, rows, reserved;
+    int32_t rows, num_caches, num_pairs, reserved;
 } pat_copy_args;
 
 int pat_b200_copy_pages(const pat_copy_args* args, void* stream);
@@ -386,7 +387,7 @@ int pat_b200_copy_pages(const pat_copy_args* args, void* stream);
  * one candidate, pad_token with its score unchanged.  A beam whose score is not finite, or whose
  * logits hold a NaN or +inf or nothing but -inf, takes no part: its candidates count as -inf, like
  * masked tokens; they fill the end of the list, lowest index first, where an entry has fewer finite
- * values than num_out.  num_out <= 128, beams <= 512, beams * ceil(vocab / 8192) <= 8192.
+ * values than num_out.  num_out <= 128, beams <= 512, vocab <= 2^24.
  * ------------------------------------------------------------------------- */
 enum { PAT_DTYPE_FP32 = 2 };
 
@@ -397,13 +398,13 @@ typedef struct pat_beam_args {
     float* out_scores;              /* [batch, num_out], contiguous */
     int32_t* out_parents;           /* beam each candidate extends */
     int32_t* out_tokens;
+    void* workspace;                /* scratch of the call, 16-byte aligned; nothing in it has to hold a value */
+    size_t workspace_bytes;
     int64_t logits_batch_stride, logits_beam_stride;    /* elements */
     int64_t scores_batch_stride, finished_batch_stride;
     int32_t batch, beams, vocab, num_out;
     int32_t dtype;                  /* PAT_DTYPE_FP16 / BF16 / FP32 */
     int32_t pad_token;
-    void* workspace;                /* scratch of the call, 16-byte aligned; nothing in it has to hold a value */
-    size_t workspace_bytes;
 } pat_beam_args;
 
 size_t pat_b200_beam_workspace_bytes(int batch, int beams, int vocab, int num_out);    /* 0: sizes out of range */

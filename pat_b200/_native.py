@@ -88,34 +88,36 @@ class Int4RowsArgs(C.Structure):
 
 class DecodeInt4Args(C.Structure):
     _fields_ = [("q", C.c_void_p), ("kv_cache", C.c_void_p), ("out", C.c_void_p), ("lse_out", C.c_void_p),
+                ("work_blob", C.c_void_p), ("workspace", C.c_void_p), ("status_word", C.c_void_p),
+                ("workspace_bytes", C.c_size_t),
                 ("q_batch_stride", C.c_int64), ("q_pos_stride", C.c_int64), ("q_head_stride", C.c_int64),
                 ("out_batch_stride", C.c_int64), ("out_pos_stride", C.c_int64), ("out_head_stride", C.c_int64),
                 ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("num_pages", C.c_int64),
                 ("batch", C.c_int32), ("q_per_req", C.c_int32), ("num_q_heads", C.c_int32),
                 ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
                 ("dtype", C.c_int32), ("flags", C.c_int32), ("softmax_scale", C.c_float),
-                ("wait_limit_us", C.c_int32), ("work_blob", C.c_void_p), ("work", WorkHeader),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status_word", C.c_void_p)]
+                ("wait_limit_us", C.c_int32), ("work", WorkHeader)]
 
 
 class CopyArgs(C.Structure):
     _fields_ = [("caches", C.c_void_p), ("host_pairs", C.c_void_p), ("device_pairs", C.c_void_p),
                 ("page_stride", C.c_int64), ("row_stride", C.c_int64), ("row_bytes", C.c_int64),
-                ("num_pages", C.c_int64), ("num_caches", C.c_int32), ("num_pairs", C.c_int32),
-                ("rows", C.c_int32), ("reserved", C.c_int32)]
+                ("num_pages", C.c_int64), ("rows", C.c_int32), ("num_caches", C.c_int32),
+                ("num_pairs", C.c_int32), ("reserved", C.c_int32)]
 
 
 class BeamArgs(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("scores", C.c_void_p), ("finished", C.c_void_p),
                 ("out_scores", C.c_void_p), ("out_parents", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
                 ("logits_batch_stride", C.c_int64), ("logits_beam_stride", C.c_int64),
                 ("scores_batch_stride", C.c_int64), ("finished_batch_stride", C.c_int64),
                 ("batch", C.c_int32), ("beams", C.c_int32), ("vocab", C.c_int32), ("num_out", C.c_int32),
-                ("dtype", C.c_int32), ("pad_token", C.c_int32),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+                ("dtype", C.c_int32), ("pad_token", C.c_int32)]
 
 
-# name -> (restype, argtypes); also the list of symbols the header declares.
+# name -> (restype, argtypes); also the list of symbols the header declares.  (An argument structure
+# declared as void* may be passed as packed bytes.)
 SIGNATURES = {
     "pat_b200_strerror": (C.c_char_p, [C.c_int]),
     "pat_b200_abi_version": (C.c_int, []),
@@ -152,12 +154,12 @@ SIGNATURES = {
     "pat_b200_reorder_heads": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "pat_b200_append_kv": (C.c_int, [C.POINTER(AppendArgs), C.c_void_p]),
     "pat_b200_int4_tile_bytes": (C.c_size_t, [C.c_int]),
-    "pat_b200_append_int4": (C.c_int, [C.POINTER(Int4RowsArgs), C.c_void_p]),
-    "pat_b200_gather_int4": (C.c_int, [C.POINTER(Int4RowsArgs), C.c_void_p]),
-    "pat_b200_decode_int4": (C.c_int, [C.POINTER(DecodeInt4Args), C.c_void_p]),
-    "pat_b200_copy_pages": (C.c_int, [C.POINTER(CopyArgs), C.c_void_p]),
+    "pat_b200_append_int4": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "pat_b200_gather_int4": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "pat_b200_decode_int4": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "pat_b200_copy_pages": (C.c_int, [C.c_void_p, C.c_void_p]),
     "pat_b200_beam_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
-    "pat_b200_beam_select": (C.c_int, [C.POINTER(BeamArgs), C.c_void_p]),
+    "pat_b200_beam_select": (C.c_int, [C.c_void_p, C.c_void_p]),
 }
 STATIC_SCRATCH_BYTES = 32 << 20
 

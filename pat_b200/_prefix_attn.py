@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import List, Optional, Sequence, Union
 
 import numpy as np
@@ -17,6 +18,7 @@ import torch
 
 from . import _native as N
 from . import _plan_cache
+from ._launch import Signatures, launch, strides_of, struct_tail
 
 __all__ = ["prefix_attn_with_kvcache", "PrefixTreeCPP", "KernelInfo", "WorkConfig", "DeviceWork",
            "status_word", "check_status"]
@@ -56,6 +58,7 @@ def _env_config() -> WorkConfig:
 
 
 _default_config: Optional[WorkConfig] = None
+_config_epoch = 0          # changes with the default options
 
 
 def default_config() -> WorkConfig:
@@ -66,8 +69,9 @@ def default_config() -> WorkConfig:
 
 
 def set_default_config(cfg: Optional[WorkConfig]) -> None:
-    global _default_config
+    global _default_config, _config_epoch
     _default_config = cfg
+    _config_epoch += 1
 
 
 def int4_config() -> WorkConfig:
@@ -275,11 +279,13 @@ class KernelInfo:
         self._vals = None           # field values, once read
         self._device = None         # where to_gpu sent the plan
         self._work = {}
+        self._int4_calls = Signatures()         # known calls of the 4-bit op with this plan
 
     def _invalidate(self):
         """The native plan changed (a pack, or an in-place advance of the tree)."""
         self._vals = None
         self._work = {}
+        self._int4_calls.clear()
 
     def __getattr__(self, name):
         if name in KernelInfo._FIELDS:
@@ -558,6 +564,7 @@ class PrefixTreeCPP:
             return False
         self._packed = False
         info._vals = None                       # the plan is stale; the work list was advanced with the tree
+        info._int4_calls.clear()                # they hold the old header
         if works:
             works[0].refresh()
         return True
@@ -837,70 +844,10 @@ def prefix_attn_with_kvcache(*args, **kwargs) -> None:
         _run(q, k_cache, v_cache, work, scale, out, lse_out, status, flags, wait_limit_us)
 
 
-def _strides(t: torch.Tensor):
-    """Strides with those of one-element dimensions, which nobody uses and torch leaves arbitrary, set to
-    the dense ones."""
-    out, dense = list(t.stride()), 1
-    for i in reversed(range(t.dim())):
-        if t.shape[i] <= 1:
-            out[i] = dense
-        dense = max(dense, out[i] * t.shape[i])
-    return out
+_INT4_POINTERS = struct.Struct("7P")
 
 
-def _run_int4(q, kv_cache, work: DeviceWork, scale: float, out, lse_out, status, flags, wait_limit_us):
-    lib = N.load()
-    stream = torch.cuda.current_stream(q.device)
-    work.order_after_upload(stream)
-    if status is None:
-        status = status_word(q.device)
-    key = (q.data_ptr(), kv_cache.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse_out is not None else 0,
-           status.data_ptr(), stream.cuda_stream, q.shape, q.stride(), kv_cache.shape, kv_cache.stride(), out.stride(),
-           q.dtype, float(scale), int(flags), int(wait_limit_us))
-    cached = work._args
-    if cached is not None and cached[0] == key:
-        a = cached[1]
-    else:
-        B, T, H, D = q.shape
-        a = N.DecodeInt4Args()
-        a.q, a.kv_cache, a.out = q.data_ptr(), kv_cache.data_ptr(), out.data_ptr()
-        a.lse_out = lse_out.data_ptr() if lse_out is not None else None
-        a.q_batch_stride, a.q_pos_stride, a.q_head_stride = _strides(q)[:3]
-        a.out_batch_stride, a.out_pos_stride, a.out_head_stride = _strides(out)[:3]
-        a.page_stride, a.head_stride = _strides(kv_cache)[:2]
-        a.num_pages = kv_cache.shape[0]
-        a.batch, a.q_per_req, a.num_q_heads, a.num_kv_heads, a.head_dim = B, T, H, kv_cache.shape[1], D
-        a.page_size = kv_cache.shape[2] * 16
-        a.dtype = _DTYPES[q.dtype]
-        a.flags = int(flags)
-        a.softmax_scale = float(scale)
-        a.wait_limit_us = int(wait_limit_us)
-        a.work_blob = work.blob.data_ptr()
-        a.work = work.header
-        need = lib.pat_b200_workspace_bytes(C.byref(work.header), H, D)
-        ws = work.workspace(need, stream, q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        a.status_word = status.data_ptr()
-        work._args = (key, a)
-    rc = lib.pat_b200_decode_int4(C.byref(a), C.c_void_p(stream.cuda_stream))
-    if rc != 0:
-        raise RuntimeError(f"prefix_attn_with_int4_kvcache failed: {N.strerror(rc)} ({rc})")
-
-
-def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree, softmax_scale: float,
-                                  out: torch.Tensor, lse_out: Optional[torch.Tensor] = None, *, _status=None,
-                                  _flags: int = 0, _wait_limit_us: int = 0) -> None:
-    """``prefix_attn_with_kvcache`` (tree form) over a KV cache held in 4 bits; writes ``out`` in place.
-
-    ``kv_cache``: uint8 ``[pages, kv_heads, page_size / 16, tile bytes]`` as ``cache_ops.int4_cache_shape``
-    gives it, filled by ``cache_ops.reshape_and_cache_int4`` with rows of ``q``'s dtype; page and head strides are
-    free.  ``tree``: a ``PrefixTreeCPP`` (or an ``AsyncTree`` holding one) whose plan was sent with
-    ``kernel_info.to_gpu(device, kv_cache_dtype="int4")``.  ``q``, ``out``, ``softmax_scale`` and ``lse_out`` are
-    those of ``prefix_attn_with_kvcache``, several query tokens per request included.  A request (or
-    position) that sees no token gets zeros, and -inf in ``lse_out``.
-
-    The products run on the exact codes; scales, offsets, softmax and sums are fp32, and the
-    probabilities are rounded to ``q``'s dtype for the second product as in the 16-bit op."""
+def _check_int4(q, kv_cache, tree, out, lse_out):
     _check(q.dtype in _DTYPES, "only support fp16 and bf16 data type")
     for t, n in ((q, "q"), (kv_cache, "kv_cache"), (out, "out")):
         _check(t.is_cuda, f"{n} must be on CUDA")
@@ -922,25 +869,82 @@ def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree,
     _check(out.dtype == q.dtype and tuple(out.shape) == tuple(q.shape), "out must be a CUDA tensor with the shape and dtype of q")
     for t, n in ((q, "q"), (out, "out")):
         _check(t.stride(-1) == 1, "Input tensor must have contiguous last dimension")
-        _check(all(s > 0 and s % 8 == 0 for s in _strides(t)[:3]) and t.data_ptr() % 16 == 0,
-               f"{n} rows must be 16-byte aligned and not overlap")
+        _check(all(s > 0 and s % 8 == 0 for s in strides_of(t)[:3]), f"{n} rows must be 16-byte aligned and not overlap")
     if lse_out is not None:
         _check(lse_out.is_cuda and lse_out.device == q.device and lse_out.dtype == torch.float32 and lse_out.is_contiguous()
                and tuple(lse_out.shape) == ((B, H) if T == 1 else (B, T, H)),
                "lse_out must be a contiguous float32 CUDA tensor [batch, heads] ([batch, seqlen_q, heads])")
-    inner = getattr(tree, "tree", None)         # an AsyncTree hands over its built tree
-    if not isinstance(tree, PrefixTreeCPP) and isinstance(inner, PrefixTreeCPP):
-        tree = inner
-    _check(isinstance(tree, PrefixTreeCPP), "tree must be a PrefixTreeCPP")
     info = tree.kernel_info
     _check(info._device is not None and info._device.type == "cuda", "the plan was not sent to the GPU (kernel_info.to_gpu)")
     _check(tree._batch() == B, f"the plan was built for {tree._batch()} requests, q has {B}")
     _check(tree._hratio == ratio, "the plan was packed for a different HRatio than q / kv_cache imply")
     _check(tree._kv_heads == Hkv, "the plan was packed for a different number of KV heads than kv_cache has")
     _check(tree.block_size == page, "the plan was built for a different page size than kv_cache has")
-    work = info.device_work(q.device, int4_config(), T)
-    with torch.cuda.device(q.device):
-        _run_int4(q, kv_cache, work, softmax_scale, out, lse_out, _status, _flags, _wait_limit_us)
+
+
+def _int4_tail(q, kv_cache, work: DeviceWork, out, scale, flags, wait_limit_us):
+    """Workspace bytes and the argument structure behind its pointers."""
+    B, T, H, D = q.shape
+    a = N.DecodeInt4Args()
+    a.q_batch_stride, a.q_pos_stride, a.q_head_stride = strides_of(q)[:3]
+    a.out_batch_stride, a.out_pos_stride, a.out_head_stride = strides_of(out)[:3]
+    a.page_stride, a.head_stride = strides_of(kv_cache)[:2]
+    a.num_pages = kv_cache.shape[0]
+    a.batch, a.q_per_req, a.num_q_heads, a.num_kv_heads, a.head_dim = B, T, H, kv_cache.shape[1], D
+    a.page_size = kv_cache.shape[2] * 16
+    a.dtype = _DTYPES[q.dtype]
+    a.flags = int(flags)
+    a.softmax_scale = float(scale)
+    a.wait_limit_us = int(wait_limit_us)
+    a.work = work.header
+    a.workspace_bytes = N.load().pat_b200_workspace_bytes(C.byref(work.header), H, D)
+    return a.workspace_bytes, struct_tail(a, _INT4_POINTERS.size)
+
+
+def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree, softmax_scale: float,
+                                  out: torch.Tensor, lse_out: Optional[torch.Tensor] = None, *, _status=None,
+                                  _flags: int = 0, _wait_limit_us: int = 0) -> None:
+    """``prefix_attn_with_kvcache`` (tree form) over a KV cache held in 4 bits; writes ``out`` in place.
+
+    ``kv_cache``: uint8 ``[pages, kv_heads, page_size / 16, tile bytes]`` as ``cache_ops.int4_cache_shape``
+    gives it, filled by ``cache_ops.reshape_and_cache_int4`` with rows of ``q``'s dtype; page and head strides are
+    free.  ``tree``: a ``PrefixTreeCPP`` (or an ``AsyncTree`` holding one) whose plan was sent with
+    ``kernel_info.to_gpu(device, kv_cache_dtype="int4")``.  ``q``, ``out``, ``softmax_scale`` and ``lse_out`` are
+    those of ``prefix_attn_with_kvcache``, several query tokens per request included.  A request (or
+    position) that sees no token gets zeros, and -inf in ``lse_out``.
+
+    The products run on the exact codes; scales, offsets, softmax and sums are fp32, and the
+    probabilities are rounded to ``q``'s dtype for the second product as in the 16-bit op."""
+    if not isinstance(tree, PrefixTreeCPP):
+        tree = getattr(tree, "tree", None)      # an AsyncTree hands over its built tree
+        _check(isinstance(tree, PrefixTreeCPP), "tree must be a PrefixTreeCPP")
+    index = q.get_device()
+    # What depends on types, shapes, strides and devices alone is checked once per work list.
+    sig = (q.dtype, q.shape, q.stride(), index, kv_cache.dtype, kv_cache.shape, kv_cache.stride(), kv_cache.get_device(),
+           out.dtype, out.shape, out.stride(), out.get_device(), softmax_scale, _flags, _wait_limit_us, _config_epoch)
+    if lse_out is not None:
+        sig += (lse_out.dtype, lse_out.shape, lse_out.stride(), lse_out.get_device())
+    info = tree.kernel_info
+    known = info._int4_calls.get(sig)
+    if known is None:
+        _check_int4(q, kv_cache, tree, out, lse_out)
+        work = info.device_work(q.device, int4_config(), q.shape[1])
+        known = info._int4_calls.remember(sig, (work, *_int4_tail(q, kv_cache, work, out, softmax_scale, _flags, _wait_limit_us)))
+    work, need, tail = known
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    ws = work._scratch.get(stream)
+    if stream != work._upload_stream or ws is None or ws.numel() < need:
+        current = torch.cuda.current_stream(index)
+        work.order_after_upload(current)
+        ws = work.workspace(need, current, q.device)
+    if _status is None:
+        _status = status_word(q.device)
+    rc = launch(N.load().pat_b200_decode_int4,
+                _INT4_POINTERS.pack(q.data_ptr(), kv_cache.data_ptr(), out.data_ptr(),
+                                    lse_out.data_ptr() if lse_out is not None else 0, work.blob.data_ptr(), ws.data_ptr(),
+                                    _status.data_ptr()) + tail, index)
+    if rc != 0:
+        raise RuntimeError(f"prefix_attn_with_int4_kvcache failed: {N.strerror(rc)} ({rc})")
 
 
 def last_launch_count() -> int:

@@ -6,13 +6,14 @@ host bookkeeping like the radix tree, since the plan of a step is made on the ho
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from . import _native as N
+from ._launch import Signatures, launch, strides_of, struct_tail
 
 _LOGIT_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -30,7 +31,40 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int, finish
     first, ties to the lower beam, then the lower token.  A beam whose score is not finite (the beams
     beyond the first of a search that starts), or whose logits hold a NaN or +inf or nothing but -inf, takes no
     part; where an entry has fewer finite values than ``num_out``, -inf entries follow, lowest beam and
-    token first.  ``num_out`` <= 128, ``beams`` <= 512, ``beams * ceil(vocab / 8192)`` <= 8192."""
+    token first.  ``num_out`` <= 128, ``beams`` <= 512, ``vocab`` <= 2^24."""
+    sig = (logits.dtype, logits.shape, logits.stride(), logits.get_device(), scores.dtype, scores.shape, scores.stride(),
+           scores.get_device(), num_out, pad_token)
+    if finished is not None:
+        sig += (finished.dtype, finished.shape, finished.stride(), finished.get_device())
+    known = _beam_calls.get(sig)
+    if known is None:
+        known = _beam_calls.remember(sig, _check_beam(logits, scores, num_out, finished, pad_token))
+    tail, index, shape, need, dense_scores, dense_finished = known
+    dev = logits.device
+    out_scores = torch.empty(shape, dtype=torch.float32, device=dev)
+    out_parents = torch.empty(shape, dtype=torch.int32, device=dev)
+    out_tokens = torch.empty(shape, dtype=torch.int32, device=dev)
+    if shape[0] == 0:
+        return out_scores, out_parents, out_tokens
+    if not dense_scores:
+        scores = scores.contiguous()
+    if not dense_finished:
+        finished = finished.contiguous()
+    # (scratch of this call alone; inside a stream capture it belongs to the graph)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    rc = launch(N.load().pat_b200_beam_select,
+                _BEAM_POINTERS.pack(logits.data_ptr(), scores.data_ptr(), finished.data_ptr() if finished is not None else 0,
+                                    out_scores.data_ptr(), out_parents.data_ptr(), out_tokens.data_ptr(), ws.data_ptr()) + tail, index)
+    if rc != 0:
+        raise RuntimeError(f"beam_select failed: {N.strerror(rc)} ({rc})")
+    return out_scores, out_parents, out_tokens
+
+
+_BEAM_POINTERS = struct.Struct("7P")
+_beam_calls = Signatures()
+
+
+def _check_beam(logits, scores, num_out, finished, pad_token):
     for name, t in (("logits", logits), ("scores", scores), ("finished", finished)):
         if t is None:
             continue
@@ -49,43 +83,25 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int, finish
         raise RuntimeError("finished must be bool [batch, beams]")
     if beams < 1 or vocab < 1:
         raise RuntimeError("logits must hold at least one beam and one token")
-    num_out, pad_token = int(num_out), int(pad_token)
-    if not 1 <= num_out <= beams * vocab:
+    if not 1 <= int(num_out) <= beams * vocab:
         raise RuntimeError("num_out must be between 1 and beams * vocab")
-    if not 0 <= pad_token < vocab:
+    if not 0 <= int(pad_token) < vocab:
         raise RuntimeError("pad_token must be a token of the vocabulary")
     if vocab > 1 and logits.stride(2) != 1:
         raise RuntimeError("logits must have a contiguous last dimension")
-    scores = scores if beams == 1 or scores.stride(1) == 1 else scores.contiguous()
-    if finished is not None and beams > 1 and finished.stride(1) != 1:
-        finished = finished.contiguous()
-    dev = logits.device
-    out = (torch.empty(batch, num_out, dtype=torch.float32, device=dev),
-           torch.empty(batch, num_out, dtype=torch.int32, device=dev),
-           torch.empty(batch, num_out, dtype=torch.int32, device=dev))
-    if batch == 0:
-        return out
-    lib = N.load()
-    need = lib.pat_b200_beam_workspace_bytes(batch, beams, vocab, num_out)
+    need = N.load().pat_b200_beam_workspace_bytes(max(batch, 1), beams, vocab, int(num_out))
     if need == 0:
-        raise RuntimeError("beam_select supports num_out <= 128, beams <= 512 and beams * ceil(vocab / 8192) <= 8192")
-    # (scratch of this call alone; inside a stream capture it belongs to the graph)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        raise RuntimeError("beam_select supports num_out <= 128, beams <= 512 and vocab <= 2^24")
+    dense_scores = beams == 1 or scores.stride(1) == 1
+    dense_finished = finished is None or beams == 1 or finished.stride(1) == 1
     a = N.BeamArgs()
-    a.logits, a.scores = logits.data_ptr(), scores.data_ptr()
-    a.finished = finished.data_ptr() if finished is not None else None
-    a.out_scores, a.out_parents, a.out_tokens = (t.data_ptr() for t in out)
-    a.logits_batch_stride, a.logits_beam_stride = logits.stride(0), logits.stride(1)
-    a.scores_batch_stride = scores.stride(0)
-    a.finished_batch_stride = finished.stride(0) if finished is not None else 0
-    a.batch, a.beams, a.vocab, a.num_out = batch, beams, vocab, num_out
-    a.dtype, a.pad_token = _LOGIT_DTYPES[logits.dtype], pad_token
-    a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    with torch.cuda.device(dev):
-        rc = lib.pat_b200_beam_select(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream))
-    if rc != 0:
-        raise RuntimeError(f"beam_select failed: {N.strerror(rc)} ({rc})")
-    return out
+    a.logits_batch_stride, a.logits_beam_stride = strides_of(logits)[:2]
+    a.scores_batch_stride = strides_of(scores)[0] if dense_scores else beams
+    a.finished_batch_stride = 0 if finished is None else strides_of(finished)[0] if dense_finished else beams
+    a.batch, a.beams, a.vocab, a.num_out = batch, beams, vocab, int(num_out)
+    a.dtype, a.pad_token = _LOGIT_DTYPES[logits.dtype], int(pad_token)
+    a.workspace_bytes = need
+    return struct_tail(a, _BEAM_POINTERS.size), logits.get_device(), (batch, int(num_out)), need, dense_scores, dense_finished
 
 
 class PagePool:

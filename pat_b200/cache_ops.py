@@ -8,13 +8,15 @@ PyTorch's current stream; there is no fallback.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
+import struct
 from typing import Optional, Sequence, Union
 
-import numpy as np
 import torch
 
 from . import _native as N
+from ._launch import Signatures, launch, strides_of, struct_tail
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -103,8 +105,14 @@ def _check_int4_cache(kv_cache: torch.Tensor, heads: int, dim: int) -> None:
         raise RuntimeError("the tiles of a page and head must be contiguous in kv_cache")
 
 
-def _int4_rows(name: str, fn: str, key, value, kv_cache, slot_mapping) -> None:
-    for n, t in (("key", key), ("value", value), ("kv_cache", kv_cache), ("slot_mapping", slot_mapping)):
+_ROW_POINTERS = struct.Struct("4P")
+_row_calls = Signatures()
+
+
+def _check_int4_rows(key, value, kv_cache, slots):
+    """(argument bytes behind the pointers, or None when there is nothing to do; device; whether
+    ``slots`` can be used as it is)."""
+    for n, t in (("key", key), ("value", value), ("kv_cache", kv_cache), ("slot_mapping", slots)):
         if not t.is_cuda:
             raise RuntimeError(f"{n} must be a CUDA tensor")
         if t.device != key.device:
@@ -118,27 +126,35 @@ def _int4_rows(name: str, fn: str, key, value, kv_cache, slot_mapping) -> None:
     for n, t in (("key", key), ("value", value)):
         if t.stride(-1) != 1:
             raise RuntimeError(f"{n} must have a contiguous last dimension")
-    slots = slot_mapping.flatten()
-    if slots.dtype != torch.int64:
-        slots = slots.to(torch.int64)
-    slots = slots.contiguous()
+    if slots.dtype.is_floating_point or slots.dtype.is_complex or slots.dtype == torch.bool:
+        raise RuntimeError("slot_mapping must hold integers")
     if slots.numel() < tokens:
         raise RuntimeError("slot_mapping is shorter than the number of tokens")
+    as_is = slots.dtype == torch.int64 and slots.is_contiguous()
     if kv_cache.shape[0] == 0 or tokens == 0 or heads == 0:
-        return
+        return None, key.get_device(), as_is
     a = N.Int4RowsArgs()
-    a.key, a.value, a.cache, a.slot_mapping = key.data_ptr(), value.data_ptr(), kv_cache.data_ptr(), slots.data_ptr()
-    # (a dimension of one element has a stride nobody uses, and torch may report any)
-    a.key_token_stride, a.value_token_stride = (t.stride(0) if tokens > 1 else heads * dim for t in (key, value))
-    a.key_head_stride, a.value_head_stride = (t.stride(1) if heads > 1 else dim for t in (key, value))
-    a.page_stride = kv_cache.stride(0) if kv_cache.shape[0] > 1 else kv_cache[0].numel()
-    a.head_stride = kv_cache.stride(1) if heads > 1 else kv_cache.shape[2] * kv_cache.shape[3]
+    (a.key_token_stride, a.key_head_stride, _), (a.value_token_stride, a.value_head_stride, _) = strides_of(key), strides_of(value)
+    a.page_stride, a.head_stride = strides_of(kv_cache)[:2]
     a.num_pages = kv_cache.shape[0]
     a.num_tokens, a.num_kv_heads, a.head_dim, a.page_size = tokens, heads, dim, kv_cache.shape[2] * 16
     a.dtype = _DTYPES[key.dtype]
-    with torch.cuda.device(key.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        rc = getattr(N.load(), fn)(C.byref(a), C.c_void_p(stream))
+    return struct_tail(a, _ROW_POINTERS.size), key.get_device(), as_is
+
+
+def _int4_rows(name: str, fn, key, value, kv_cache, slots) -> None:
+    sig = (key.dtype, key.shape, key.stride(), key.get_device(), value.dtype, value.shape, value.stride(), value.get_device(),
+           kv_cache.dtype, kv_cache.shape, kv_cache.stride(), kv_cache.get_device(),
+           slots.dtype, slots.shape, slots.stride(), slots.get_device())
+    known = _row_calls.get(sig)
+    if known is None:
+        known = _row_calls.remember(sig, _check_int4_rows(key, value, kv_cache, slots))
+    tail, index, as_is = known
+    if tail is None:
+        return
+    if not as_is:
+        slots = slots.flatten().to(torch.int64).contiguous()
+    rc = launch(fn, _ROW_POINTERS.pack(key.data_ptr(), value.data_ptr(), kv_cache.data_ptr(), slots.data_ptr()) + tail, index)
     if rc != 0:
         raise RuntimeError(f"{name} failed: {N.strerror(rc)} ({rc})")
 
@@ -149,14 +165,14 @@ def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_cache: tor
     cache (``int4_cache_shape``) at ``slot_mapping[i] = page * page_size + row``.  Tokens with a
     negative slot, or one beyond the cache, are skipped; slots must be distinct.  A row that holds a NaN or an
     infinity is stored as NaN.  All rows of a cache have one dtype (its scales are stored in it)."""
-    _int4_rows("reshape_and_cache_int4", "pat_b200_append_int4", key, value, kv_cache, slot_mapping)
+    _int4_rows("reshape_and_cache_int4", N.load().pat_b200_append_int4, key, value, kv_cache, slot_mapping)
 
 
 def gather_cache_int4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> None:
     """Reads the tokens at ``slot_mapping`` back from a 4-bit cache into ``key`` / ``value``
     (``[num_tokens, kv_heads, head_dim]``, the dtype that was appended), e.g. a cached prefix for a
     prefill that runs on 16-bit keys.  Rows of skipped slots (see ``reshape_and_cache_int4``) keep what they hold."""
-    _int4_rows("gather_cache_int4", "pat_b200_gather_int4", key, value, kv_cache, slot_mapping)
+    _int4_rows("gather_cache_int4", N.load().pat_b200_gather_int4, key, value, kv_cache, slot_mapping)
 
 
 # --------------------------------------------------------------------------- moving pages
@@ -189,12 +205,13 @@ def copy_pages(caches: Union[torch.Tensor, Sequence[torch.Tensor]], mapping) -> 
     of one pair may occur in another), or an int64 CUDA tensor with the same contract, which is not
     checked; pairs with a page outside the cache are then skipped.  A host mapping travels in the
     launch itself: a CUDA graph captured around the call repeats that mapping."""
-    caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
+    caches = [caches] if isinstance(caches, torch.Tensor) else caches
     on_device = isinstance(mapping, torch.Tensor) and mapping.is_cuda
     if not on_device:
-        mapping = torch.as_tensor(mapping, dtype=torch.int64).contiguous()
+        mapping = torch.as_tensor(mapping, dtype=torch.int64)
         if mapping.numel() == 0:
             mapping = mapping.reshape(0, 2)
+        mapping = mapping.contiguous()
     if mapping.dim() != 2 or mapping.shape[1] != 2:
         raise RuntimeError("mapping must be [n, 2]: pairs (from, to)")
     if on_device and (mapping.dtype != torch.int64 or not mapping.is_contiguous()):
@@ -202,45 +219,57 @@ def copy_pages(caches: Union[torch.Tensor, Sequence[torch.Tensor]], mapping) -> 
     if not caches:
         return
     first = caches[0]
+    shape, strides, dtype, index = first.shape, first.stride(), first.dtype, first.get_device()
     for t in caches:
-        if not t.is_cuda:
+        if t.get_device() < 0:
             raise RuntimeError("caches must be CUDA tensors")
-        if t.device != first.device or t.dtype != first.dtype or t.shape != first.shape or t.stride() != first.stride():
+        if t.get_device() != index or t.dtype != dtype or t.shape != shape or t.stride() != strides:
             raise RuntimeError("caches must share device, dtype, shape and strides")
-    if on_device and mapping.device != first.device:
+    if on_device and mapping.get_device() != index:
         raise RuntimeError("mapping must be on the device of the caches, or on the host")
-    if first.dim() < 2:
-        raise RuntimeError("caches must be [pages, ...]")
-    pages = first.shape[0]
-    n = mapping.shape[0]
-    if not on_device and n:
-        src, dst = mapping[:, 0], mapping[:, 1]
-        if int(mapping.min()) < 0 or int(mapping.max()) >= pages:
-            raise RuntimeError(f"mapping names a page outside the cache ({pages} pages)")
-        flat = dst.numpy()
-        hit = np.zeros(pages, dtype=np.int32)
-        np.add.at(hit, flat, 1)
-        if hit.max() > 1:
-            raise RuntimeError("a page is the target of two pairs")
-        if hit[src.numpy()].any():
-            raise RuntimeError("a page is both a source and a target")
-    if n == 0 or first.numel() == 0:
-        return
-    geometry = _page_geometry(first)
+    sig = (shape, strides, dtype)
+    geometry = _copy_geometries.get(sig)
     if geometry is None:
-        raise RuntimeError("a page must consist of equally long contiguous runs at one stride")
-    a = N.CopyArgs()
-    ptrs = (C.c_void_p * len(caches))(*[t.data_ptr() for t in caches])
-    a.caches = C.cast(ptrs, C.c_void_p)
-    if on_device:
-        a.device_pairs = mapping.data_ptr()
-    else:
-        a.host_pairs = mapping.data_ptr()
-    a.rows, a.row_stride, a.row_bytes = geometry
-    a.page_stride = first.stride(0) * first.element_size() if pages > 1 else a.rows * a.row_stride
-    a.num_pages, a.num_caches, a.num_pairs = pages, len(caches), n
-    with torch.cuda.device(first.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        rc = N.load().pat_b200_copy_pages(C.byref(a), C.c_void_p(stream))
+        geometry = _copy_geometries.remember(sig, _copy_geometry(first))
+    n = mapping.shape[0]
+    if geometry is _NO_BYTES:
+        if n and shape[0] == 0:
+            raise RuntimeError("mapping names a page outside the cache (0 pages)")
+        return
+    pointers = array.array("Q", [t.data_ptr() for t in caches])
+    address = mapping.data_ptr() if n else 0
+    rc = launch(N.load().pat_b200_copy_pages,
+                _COPY_ARGS.pack(pointers.buffer_info()[0], 0 if on_device else address, address if on_device else 0, *geometry,
+                                len(pointers), n, 0), index)
+    if rc == -10:
+        _explain_mapping(mapping, shape[0])
     if rc != 0:
         raise RuntimeError(f"copy_pages failed: {N.strerror(rc)} ({rc})")
+
+
+_COPY_ARGS = struct.Struct("3P4q4i")        # pat_copy_args, `rows` first of the int32
+_copy_geometries = Signatures()
+_NO_BYTES = ()
+
+
+def _copy_geometry(cache: torch.Tensor):
+    """(page_stride, row_stride, row_bytes, num_pages, rows) of the argument structure."""
+    if cache.dim() < 2:
+        raise RuntimeError("caches must be [pages, ...]")
+    if cache.numel() == 0:
+        return _NO_BYTES
+    geometry = _page_geometry(cache)
+    if geometry is None:
+        raise RuntimeError("a page must consist of equally long contiguous runs at one stride")
+    rows, row_stride, row_bytes = geometry
+    page_stride = cache.stride(0) * cache.element_size() if cache.shape[0] > 1 else rows * row_stride
+    return page_stride, row_stride, row_bytes, cache.shape[0], rows
+
+
+def _explain_mapping(mapping: torch.Tensor, pages: int) -> None:
+    """Says what is wrong with a mapping the library refused."""
+    if int(mapping.min()) < 0 or int(mapping.max()) >= pages:
+        raise RuntimeError(f"mapping names a page outside the cache ({pages} pages)")
+    if mapping[:, 1].unique().numel() != mapping.shape[0]:
+        raise RuntimeError("a page is the target of two pairs")
+    raise RuntimeError("a page is both a source and a target")

@@ -4,11 +4,12 @@
 // the num_out largest values of an entry, larger first, ties to the lower k * vocab + v.  (The
 // reference has no sampling; its serving engine does that.)
 //
-// Two kernels.  beam_scan reads the logits once: a CTA takes 8192 consecutive logits of a row into
+// Two kernels.  beam_scan reads the logits once: a CTA takes up to 8192 consecutive logits of a row into
 // registers, sums their exponentials against the chunk's maximum, and lists the chunk's num_out largest.
 // Inside a beam the order of the values is the order of the logits, so the lists need no softmax.
-// beam_pick has one CTA per entry: it joins the chunks' sums, and draws num_out times the largest of
-// the heads of the lists.
+// beam_pick, its programmatic dependent, has one CTA per entry: it joins the chunks' sums and picks the
+// num_out best of the lists.  Both find a lower bound of the num_out-th largest from the threads' maxima -
+// every warp sorts its 32 - collect the few that reach it, and order those by counting.
 //
 // Candidates of different beams are compared by a value that contains two log-sums, so these are
 // kept to about 1e-8: exponentials in fp32 with the argument in two parts, sums of at most 32 of them
@@ -27,10 +28,11 @@ namespace {
 
 constexpr uint32_t kFull = 0xffffffffu;
 constexpr int kThreads = 256;
-constexpr int kGroups = 4;                         // groups of 8 consecutive logits per thread
-constexpr int kPer = kGroups * 8;
-constexpr int kChunk = kThreads * kPer;            // 8192
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxGroups = 4;                      // groups of 8 consecutive logits per thread
 constexpr int kMaxOut = 128;
+constexpr int kMaxBeams = 512;
+static_assert(2 * kMaxOut == kThreads, "s_used is cleared by one store per thread");
 constexpr int kListCap = 1024;
 
 struct BeamParams {
@@ -48,7 +50,7 @@ struct BeamParams {
     int32_t* list_n;               // [rows][chunks]
     float* chunk_max;
     double* chunk_sum;
-    int batch, beams, vocab, num_out, chunks, pad_token;
+    int batch, beams, vocab, num_out, chunks, chunk_len, pad_token;
 };
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
@@ -91,7 +93,23 @@ __device__ __forceinline__ bool beam_is_live(const BeamParams& p, int64_t b, int
     return isfinite(p.scores[b * p.score_stride + k]);
 }
 
-template <typename T> __global__ void __launch_bounds__(kThreads) beam_scan_kernel(const BeamParams p) {
+// The values of the warp's lanes in descending order (bitonic sort): lane i gets the (i + 1)-th largest.
+__device__ __forceinline__ float warp_sorted(float v, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+        for (int d = size / 2; d > 0; d >>= 1) {
+            const float o = __shfl_xor_sync(kFull, v, d);
+            const bool keep_max = ((lane & size) == 0) == ((lane & d) == 0);
+            v = keep_max ? fmaxf(v, o) : fminf(v, o);
+        }
+    }
+    return v;
+}
+
+template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 3) beam_scan_kernel(const BeamParams p) {
+    constexpr int kPer = kGroups * 8;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int64_t row = blockIdx.x / p.chunks;
     const int chunk = static_cast<int>(blockIdx.x - row * p.chunks);
     const int64_t b = row / p.beams;
@@ -99,29 +117,27 @@ template <typename T> __global__ void __launch_bounds__(kThreads) beam_scan_kern
     if (!beam_is_live(p, b, k)) return;            // nobody reads this row's lists
     const T* src = static_cast<const T*>(p.logits) + b * p.batch_stride + static_cast<int64_t>(k) * p.beam_stride;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int kWarps = kThreads / 32;
-    __shared__ float s_top[kThreads];
-    __shared__ float s_red[kWarps];
+    __shared__ float s_max[kWarps], s_edge[kWarps];
     __shared__ double s_sum[kWarps];
-    __shared__ int s_bad, s_count;
+    __shared__ int s_bad[kWarps], s_count;
     __shared__ float s_x[kListCap];
     __shared__ int s_v[kListCap];
-    if (tid == 0) { s_bad = 0; s_count = 0; }
+    if (tid == 0) s_count = 0;
 
-    // logits past the end of the row, and -inf ones, are no candidates and add nothing to the sum
+    // logits past the end of the chunk, and -inf ones, are no candidates and add nothing to the sum
     float x[kPer];
-    const int base = chunk * kChunk;
+    const int base = chunk * p.chunk_len, end = min(base + p.chunk_len, p.vocab);
 #pragma unroll
     for (int gi = 0; gi < kGroups; ++gi) {
         const int at = base + gi * (kThreads * 8) + tid * 8;
-        if (at + 8 <= p.vocab) {
+        if (at + 8 <= end) {
             float y[8];
             load8<T>(src + at, y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[gi * 8 + i] = y[i];
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[gi * 8 + i] = at + i < p.vocab ? to_float<T>(src[at + i]) : -INFINITY;
+            for (int i = 0; i < 8; ++i) x[gi * 8 + i] = at + i < end ? to_float<T>(src[at + i]) : -INFINITY;
         }
     }
     auto token_of = [&](int i) { return base + (i >> 3) * (kThreads * 8) + tid * 8 + (i & 7); };
@@ -132,45 +148,32 @@ template <typename T> __global__ void __launch_bounds__(kThreads) beam_scan_kern
         top = fmaxf(top, x[i]);
         bad = bad || !(x[i] < INFINITY);           // NaN or +inf: the beam takes no part
     }
-    s_top[tid] = top;
-    float m = top;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
-    if (lane == 0) s_red[warp] = m;
+    // At least q of every warp's maxima reach `edge`, so at least num_out logits of the chunk do.
+    const int q = (p.num_out + kWarps - 1) / kWarps;
+    const float sorted = warp_sorted(top, lane);
+    const bool any_bad = __any_sync(kFull, bad);
+    if (lane == 0) { s_max[warp] = sorted; s_bad[warp] = any_bad; }
+    if (lane == q - 1) s_edge[warp] = sorted;
     __syncthreads();
-    if (__any_sync(kFull, bad) && lane == 0) s_bad = 1;
-    m = s_red[0];
+    float m = s_max[0], edge = s_edge[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_red[w]);
+    for (int w = 1; w < kWarps; ++w) { m = fmaxf(m, s_max[w]); edge = fminf(edge, s_edge[w]); }
 
     float sum = 0.f;
     if (m > -INFINITY) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += exp_neg(x[i] - m);
+        for (int i = 0; i < kPer; ++i) {
+            sum += exp_neg(x[i] - m);
+            if (x[i] >= edge && x[i] > -INFINITY) {
+                const int at = atomicAdd(&s_count, 1);
+                if (at < kListCap) { s_x[at] = x[i]; s_v[at] = token_of(i); }
+            }
+        }
     }
     double total = sum;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(kFull, total, d);
     if (lane == 0) s_sum[warp] = total;
-
-    // The num_out-th largest of the threads' maxima is a lower bound of the num_out-th largest logit:
-    // only what reaches it can be among the num_out largest.
-    int rank = 0;
-    for (int i = 0; i < kThreads; ++i) {
-        const float o = s_top[i];
-        rank += (o > top || (o == top && i < tid)) ? 1 : 0;
-    }
-    __syncthreads();                               // (also: everyone has read s_red)
-    if (rank == p.num_out - 1) s_red[0] = top;     // exactly one thread has this rank
-    __syncthreads();
-    const float edge = s_red[0];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        if (x[i] > -INFINITY && x[i] >= edge) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kListCap) { s_x[at] = x[i]; s_v[at] = token_of(i); }
-        }
-    }
     __syncthreads();
     const int found = s_count;
     const size_t slot = static_cast<size_t>(row) * p.chunks + chunk;
@@ -178,8 +181,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads) beam_scan_kern
     int32_t* out_v = p.list_v + slot * p.num_out;
     if (tid == 0) {
         double z = 0.0;
-        for (int w = 0; w < kWarps; ++w) z += s_sum[w];
-        p.chunk_max[slot] = s_bad ? NAN : m;
+        int any = 0;
+        for (int w = 0; w < kWarps; ++w) { z += s_sum[w]; any |= s_bad[w]; }
+        p.chunk_max[slot] = any ? NAN : m;
         p.chunk_sum[slot] = z;
         p.list_n[slot] = found < p.num_out ? found : p.num_out;
     }
@@ -193,7 +197,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) beam_scan_kern
         }
         return;
     }
-    // Many equal logits: draw the largest remaining one num_out times.
+    // Very many equal logits, or maxima in few warps only: draw the largest remaining one num_out times.
     uint32_t taken = 0;
     for (int n = 0; n < p.num_out; ++n) {
         float bx = -INFINITY;
@@ -211,6 +215,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) beam_scan_kern
             const int ov = __shfl_xor_sync(kFull, wv, d);
             if (before(ox, ov, wx, wv)) { wx = ox; wv = ov; }
         }
+        __syncthreads();                           // (everyone has read the lists / the last round)
         if (lane == 0) { s_x[warp] = wx; s_v[warp] = wv; }
         __syncthreads();
         wx = s_x[0];
@@ -218,120 +223,169 @@ template <typename T> __global__ void __launch_bounds__(kThreads) beam_scan_kern
         for (int w = 1; w < kWarps; ++w)
             if (before(s_x[w], s_v[w], wx, wv)) { wx = s_x[w]; wv = s_v[w]; }
         if (bi >= 0 && bv == wv) { taken |= 1u << bi; out_x[n] = wx; out_v[n] = wv; }
-        __syncthreads();
     }
 }
+
+__device__ __forceinline__ bool before(double xa, int64_t ia, double xb, int64_t ib) { return xa > xb || (xa == xb && ia < ib); }
 
 __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p) {
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int kWarps = kThreads / 32;
-    const int lists = p.beams * p.chunks;          // heads of all lists, plus one entry per finished beam
-    extern __shared__ double s_shift[];            // [beams] score - log-sum, or NaN: the beam takes no part
-    int* s_cursor = reinterpret_cast<int*>(s_shift + p.beams);      // [lists]
-    __shared__ double s_val[kWarps];
-    __shared__ int64_t s_idx[kWarps];
-    __shared__ int s_list[kWarps];
-    __shared__ int64_t s_chosen[kMaxOut];
+    __shared__ double s_shift[kMaxBeams];          // score - log-sum; NaN: the beam takes no part
+    __shared__ float s_edge[kWarps];
+    __shared__ double s_val[kListCap];
+    __shared__ int64_t s_idx[kListCap];
+    __shared__ int s_count;
+    __shared__ uint8_t s_used[2 * kMaxOut];
+    if (tid == 0) s_count = 0;
+    s_used[tid] = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    for (int k = tid; k < p.beams; k += kThreads) {
+    for (int k = warp; k < p.beams; k += kWarps) {
         double shift = NAN;
         if (beam_is_live(p, b, k)) {
             const size_t slot = (static_cast<size_t>(b) * p.beams + k) * p.chunks;
             float m = -INFINITY;
             bool bad = false;
-            for (int c = 0; c < p.chunks; ++c) {
+            for (int c = lane; c < p.chunks; c += 32) {
                 const float cm = p.chunk_max[slot + c];
                 bad = bad || cm != cm;
                 m = fmaxf(m, cm);
             }
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
+            bad = __any_sync(kFull, bad);
             if (!bad && m > -INFINITY) {
                 double z = 0.0;
-                for (int c = 0; c < p.chunks; ++c) {
+                for (int c = lane; c < p.chunks; c += 32) {
                     const float cm = p.chunk_max[slot + c];
                     if (cm > -INFINITY) z += p.chunk_sum[slot + c] * exp(static_cast<double>(cm) - static_cast<double>(m));
                 }
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) z += __shfl_xor_sync(kFull, z, d);
                 shift = static_cast<double>(p.scores[b * p.score_stride + k]) - (static_cast<double>(m) + log(z));
             }
         }
-        s_shift[k] = shift;
+        if (lane == 0) s_shift[k] = shift;
     }
-    for (int i = tid; i < lists; i += kThreads) s_cursor[i] = 0;
     __syncthreads();
 
-    int n = 0;
-    for (; n < p.num_out; ++n) {
+    // Candidates: the lists' places one after the other, then one per beam for those that are finished.
+    const int64_t listed = static_cast<int64_t>(p.beams) * p.chunks * p.num_out;
+    const int64_t total = listed + p.beams;
+    auto candidate = [&](int64_t j, double& val, int64_t& idx) -> bool {
+        if (j < listed) {
+            const int64_t list = j / p.num_out;
+            const int pos = static_cast<int>(j - list * p.num_out), k = static_cast<int>(list / p.chunks);
+            const double shift = s_shift[k];
+            const size_t slot = static_cast<size_t>(b) * p.beams * p.chunks + list;
+            if (shift != shift || pos >= p.list_n[slot]) return false;
+            val = shift + static_cast<double>(p.list_x[slot * p.num_out + pos]);
+            idx = static_cast<int64_t>(k) * p.vocab + p.list_v[slot * p.num_out + pos];
+            return true;
+        }
+        const int k = static_cast<int>(j - listed);
+        if (!p.finished || !p.finished[b * p.finished_stride + k]) return false;
+        const float sc = p.scores[b * p.score_stride + k];
+        if (!isfinite(sc)) return false;
+        val = sc;
+        idx = static_cast<int64_t>(k) * p.vocab + p.pad_token;
+        return true;
+    };
+    double val;
+    int64_t idx;
+    float top = -INFINITY;
+    for (int64_t j = tid; j < total; j += kThreads)
+        if (candidate(j, val, idx)) top = fmaxf(top, __double2float_rd(val));
+    const float sorted = warp_sorted(top, lane);
+    if (lane == (p.num_out + kWarps - 1) / kWarps - 1) s_edge[warp] = sorted;
+    __syncthreads();
+    float edge = s_edge[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) edge = fminf(edge, s_edge[w]);
+    for (int64_t j = tid; j < total; j += kThreads) {
+        if (candidate(j, val, idx) && val >= static_cast<double>(edge)) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kListCap) { s_val[at] = val; s_idx[at] = idx; }
+        }
+    }
+    __syncthreads();
+    const int found = s_count;
+    auto put = [&](int n, double v, int64_t i) {
+        p.out_scores[b * p.num_out + n] = static_cast<float>(v);
+        p.out_parents[b * p.num_out + n] = static_cast<int32_t>(i / p.vocab);
+        p.out_tokens[b * p.num_out + n] = static_cast<int32_t>(i % p.vocab);
+    };
+    if (found <= kListCap) {
+        for (int i = tid; i < found; i += kThreads) {
+            const double vi = s_val[i];
+            const int64_t ii = s_idx[i];
+            int r = 0;
+            for (int j = 0; j < found; ++j) r += before(s_val[j], s_idx[j], vi, ii) ? 1 : 0;
+            if (r < p.num_out) put(r, vi, ii);
+            if (ii < 2 * kMaxOut) s_used[ii] = 1;
+        }
+        if (found >= p.num_out) return;
+        // Fewer finite values than asked for, and all of them are listed: the rest are -inf, all equal, so the
+        // lowest indices not among the listed follow.  They lie below num_out + found < 2 kMaxOut.
+        __syncthreads();
+        if (tid == 0)
+            for (int64_t i = 0, n = found; n < p.num_out; ++i)
+                if (!s_used[i]) put(static_cast<int>(n++), -INFINITY, i);
+        return;
+    }
+    // Very many equal values: num_out times the best behind the last one chosen.
+    double last = INFINITY;
+    int64_t last_idx = -1;
+    for (int n = 0; n < p.num_out; ++n) {
         double best = -INFINITY;
         int64_t best_idx = INT64_MAX;
-        int best_list = -1;
-        for (int i = tid; i < lists; i += kThreads) {
-            const int k = i / p.chunks, c = i - k * p.chunks;
-            double val;
-            int64_t idx;
-            const bool done = p.finished && p.finished[b * p.finished_stride + k];
-            if (done) {
-                if (c != 0 || s_cursor[i] > 0) continue;
-                const float sc = p.scores[b * p.score_stride + k];
-                if (!isfinite(sc)) continue;
-                val = sc;
-                idx = static_cast<int64_t>(k) * p.vocab + p.pad_token;
-            } else {
-                const double shift = s_shift[k];
-                const size_t slot = (static_cast<size_t>(b) * p.beams + k) * p.chunks + c;
-                if (shift != shift || s_cursor[i] >= p.list_n[slot]) continue;
-                val = shift + static_cast<double>(p.list_x[slot * p.num_out + s_cursor[i]]);
-                idx = static_cast<int64_t>(k) * p.vocab + p.list_v[slot * p.num_out + s_cursor[i]];
-            }
-            if (val > best || (val == best && idx < best_idx)) { best = val; best_idx = idx; best_list = i; }
-        }
-        double wv = best;
-        int64_t wi = best_idx;
-        int wl = best_list;
+        for (int64_t j = tid; j < total; j += kThreads)
+            if (candidate(j, val, idx) && before(last, last_idx, val, idx) && before(val, idx, best, best_idx)) { best = val; best_idx = idx; }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) {
-            const double ov = __shfl_xor_sync(kFull, wv, d);
-            const int64_t oi = __shfl_xor_sync(kFull, wi, d);
-            const int ol = __shfl_xor_sync(kFull, wl, d);
-            if (ov > wv || (ov == wv && oi < wi)) { wv = ov; wi = oi; wl = ol; }
+            const double ov = __shfl_xor_sync(kFull, best, d);
+            const int64_t oi = __shfl_xor_sync(kFull, best_idx, d);
+            if (before(ov, oi, best, best_idx)) { best = ov; best_idx = oi; }
         }
-        if (lane == 0) { s_val[warp] = wv; s_idx[warp] = wi; s_list[warp] = wl; }
         __syncthreads();
-        wv = s_val[0]; wi = s_idx[0]; wl = s_list[0];
+        if (lane == 0) { s_val[warp] = best; s_idx[warp] = best_idx; }
+        __syncthreads();
+        last = s_val[0];
+        last_idx = s_idx[0];
         for (int w = 1; w < kWarps; ++w)
-            if (s_val[w] > wv || (s_val[w] == wv && s_idx[w] < wi)) { wv = s_val[w]; wi = s_idx[w]; wl = s_list[w]; }
-        if (wl < 0) break;                         // uniform: nothing finite is left
-        if (tid == 0) {
-            s_cursor[wl] += 1;
-            s_chosen[n] = wi;
-            p.out_scores[b * p.num_out + n] = static_cast<float>(wv);
-            p.out_parents[b * p.num_out + n] = static_cast<int32_t>(wi / p.vocab);
-            p.out_tokens[b * p.num_out + n] = static_cast<int32_t>(wi % p.vocab);
-        }
-        __syncthreads();
+            if (before(s_val[w], s_idx[w], last, last_idx)) { last = s_val[w]; last_idx = s_idx[w]; }
+        if (tid == 0) put(n, last, last_idx);
     }
-    // Fewer finite values than asked for: the rest are -inf, all equal, so the lowest indices not
-    // chosen yet follow.  Every finite value of the entry has been chosen by now.
-    if (n < p.num_out && tid == 0) {
-        const int finite = n;
-        for (int64_t idx = 0; n < p.num_out; ++idx) {
-            bool used = false;
-            for (int i = 0; i < finite; ++i) used = used || s_chosen[i] == idx;
-            if (used) continue;
-            p.out_scores[b * p.num_out + n] = -INFINITY;
-            p.out_parents[b * p.num_out + n] = static_cast<int32_t>(idx / p.vocab);
-            p.out_tokens[b * p.num_out + n] = static_cast<int32_t>(idx % p.vocab);
-            ++n;
-        }
+}
+
+// How a row is cut.  8192 logits per CTA keep 4 x 16 bytes (or more) of every thread in flight, and lists
+// few; with less than two CTAs per SM then, shorter chunks spread the rows over more SMs.
+struct Cut { int groups, chunks, chunk_len; };
+Cut cut_rows(int64_t rows, int vocab) {
+    Cut c{kMaxGroups, 0, 0};
+    while (true) {
+        const int64_t len = static_cast<int64_t>(c.groups) * kThreads * 8;
+        const int64_t chunks = (vocab + len - 1) / len;
+        if (c.groups > 1 && rows * chunks < 2 * 148) { c.groups /= 2; continue; }
+        c.chunks = static_cast<int>(chunks);
+        c.chunk_len = static_cast<int>(((vocab + chunks - 1) / chunks + 7) / 8 * 8);       // chunks of equal length
+        c.chunks = (vocab + c.chunk_len - 1) / c.chunk_len;
+        return c;
     }
 }
 
 int beam_shape(int batch, int beams, int vocab, int num_out) {
     if (batch < 0 || beams <= 0 || vocab <= 0 || num_out <= 0) return PAT_ERR_BAD_ARGUMENT;
     if (num_out > static_cast<int64_t>(beams) * vocab) return PAT_ERR_BAD_ARGUMENT;
-    if (num_out > kMaxOut || beams > 512) return PAT_ERR_TOO_LARGE;
-    const int64_t chunks = (static_cast<int64_t>(vocab) + kChunk - 1) / kChunk;
-    if (static_cast<int64_t>(beams) * chunks > 8192 || static_cast<int64_t>(batch) * beams * chunks > 0x7fffffffLL) return PAT_ERR_TOO_LARGE;
+    if (num_out > kMaxOut || beams > kMaxBeams || vocab > (1 << 24)) return PAT_ERR_TOO_LARGE;
+    const int64_t rows = static_cast<int64_t>(batch) * beams;
+    if (rows * cut_rows(rows, vocab).chunks > 0x7fffffffLL) return PAT_ERR_TOO_LARGE;
     return PAT_OK;
+}
+
+template <typename T> void (*scan_of(int groups))(BeamParams) {
+    return groups == 4 ? beam_scan_kernel<T, 4> : groups == 2 ? beam_scan_kernel<T, 2> : beam_scan_kernel<T, 1>;
 }
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
@@ -340,7 +394,8 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 extern "C" size_t pat_b200_beam_workspace_bytes(int batch, int beams, int vocab, int num_out) {
     if (beam_shape(batch, beams, vocab, num_out) != PAT_OK) return 0;
-    const size_t lists = static_cast<size_t>(batch) * beams * ((static_cast<size_t>(vocab) + kChunk - 1) / kChunk);
+    const int64_t rows = static_cast<int64_t>(batch) * beams;
+    const size_t lists = static_cast<size_t>(rows) * cut_rows(rows, vocab).chunks;
     return 2 * align256(lists * num_out * 4) + 2 * align256(lists * 4) + align256(lists * 8);
 }
 
@@ -373,7 +428,9 @@ extern "C" int pat_b200_beam_select(const pat_beam_args* args, void* stream_hand
     p.vocab = a.vocab;
     p.num_out = a.num_out;
     p.pad_token = a.pad_token;
-    p.chunks = static_cast<int>((static_cast<int64_t>(a.vocab) + kChunk - 1) / kChunk);
+    const Cut cut = cut_rows(static_cast<int64_t>(a.batch) * a.beams, a.vocab);
+    p.chunks = cut.chunks;
+    p.chunk_len = cut.chunk_len;
     const size_t lists = static_cast<size_t>(a.batch) * a.beams * p.chunks;
     unsigned char* ws = static_cast<unsigned char*>(a.workspace);
     p.chunk_sum = reinterpret_cast<double*>(ws);
@@ -387,10 +444,21 @@ extern "C" int pat_b200_beam_select(const pat_beam_args* args, void* stream_hand
     p.chunk_max = reinterpret_cast<float*>(ws);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
     const unsigned grid = static_cast<unsigned>(lists);
-    if (a.dtype == PAT_DTYPE_FP32) beam_scan_kernel<float><<<grid, kThreads, 0, stream>>>(p);
-    else if (a.dtype == PAT_DTYPE_BF16) beam_scan_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p);
-    else beam_scan_kernel<__half><<<grid, kThreads, 0, stream>>>(p);
-    const size_t smem = static_cast<size_t>(a.beams) * 8 + static_cast<size_t>(a.beams) * p.chunks * 4;   // <= 36 KB by beam_shape
-    beam_pick_kernel<<<static_cast<unsigned>(a.batch), kThreads, smem, stream>>>(p);
+    void (*scan)(BeamParams);
+    if (a.dtype == PAT_DTYPE_FP32) scan = scan_of<float>(cut.groups);
+    else if (a.dtype == PAT_DTYPE_BF16) scan = scan_of<__nv_bfloat16>(cut.groups);
+    else scan = scan_of<__half>(cut.groups);
+    scan<<<grid, kThreads, 0, stream>>>(p);
+    // starts while the scan runs, and waits for its end before it reads anything the scan wrote
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.batch));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, beam_pick_kernel, p) != cudaSuccess) return PAT_ERR_CUDA;
     return cudaGetLastError() == cudaSuccess ? PAT_OK : PAT_ERR_CUDA;
 }

@@ -26,22 +26,56 @@ struct RowsParams {            // append and read-back: rows of 16-bit elements 
     const int64_t* slots;
     int64_t key_token, key_head, value_token, value_head;     // elements
     int64_t page_stride, head_stride;                         // bytes
-    int64_t num_slots, num_rows;                              // pages * page_size; tokens * 2 * heads
-    int heads, page_size;
+    int64_t num_slots;                                        // pages * page_size
+    int num_tokens, heads, page_size;
 };
 
-// Byte offsets, from the start of the tile, of what the thread that owns dims 8i .. 8i + 7 of token
-// `tok` reads or writes: one word of K, two 16-bit halves of V (the second 4 bytes on).
+// Byte offsets, from the start of a tile, of the codes of dims 8i .. 8i + 7 of token `tok`: one word of K,
+// two 16-bit halves of V (the second 4 bytes on).
 template <int D> __device__ __forceinline__ int k_word_off(int tok, int i) { return tok * Int4Tile<D>::kTokenBytes + i * 4; }
 template <int D> __device__ __forceinline__ int v_half_off(int tok, int i) {
-    constexpr int kThreadsPerLane = D / 64;                   // 16-byte pieces of a row per V lane
-    const int g = i / kThreadsPerLane, wh = i - g * kThreadsPerLane;
+    constexpr int kPerLane = D / 64;                          // groups of 8 dims per V lane
+    const int g = i / kPerLane, wh = i - g * kPerLane;
     return Int4Tile<D>::kVOff + (tok >> 3) * 4 * D + (g * 4 + ((tok & 7) >> 1)) * Int4Tile<D>::kLaneBytes + wh * 8 + (tok & 1) * 2;
 }
 
-// Address of the tile of (slot, head), or null for a padding slot / a slot outside the cache.
+// Both kernels: one CTA = 16 consecutive tokens of the call x one KV head (heads next to each other: they
+// share the tokens' rows).  When the 16 slots are one tile in order - a prefill chunk, a cached prefix - the
+// tile passes through shared memory and is moved by 16-byte accesses; otherwise every row goes to its place by
+// itself, V in 2-byte pieces (a token owns 16-bit halves of the V words).
+constexpr int kRowThreads = 256;
+
+struct TileGroup {
+    int64_t slot[16];          // -1: padding, or outside the cache
+    unsigned char* tile;       // the one tile of a whole run, or null
+};
+
+// All threads call this; `grp` is shared memory.
+template <int D> __device__ __forceinline__ void load_group(const RowsParams& p, TileGroup& grp, int token0, int head) {
+    if (threadIdx.x < 32) {
+        const int t = threadIdx.x;
+        int64_t slot = -1;
+        if (t < 16 && token0 + t < p.num_tokens) {
+            slot = __ldg(p.slots + token0 + t);
+            if (slot < 0 || slot >= p.num_slots) slot = -1;
+        }
+        const int64_t first = __shfl_sync(kFullMask, slot, 0);
+        const bool run = __all_sync(kFullMask, t >= 16 || (first >= 0 && slot == first + t)) && (first & 15) == 0;
+        if (t < 16) grp.slot[t] = slot;
+        if (t == 0) {
+            unsigned char* tile = nullptr;
+            if (run) {
+                const int64_t page = first / p.page_size;
+                tile = p.cache + page * p.page_stride + head * p.head_stride +
+                       ((first - page * p.page_size) >> 4) * Int4Tile<D>::kBytes;
+            }
+            grp.tile = tile;
+        }
+    }
+    __syncthreads();
+}
+
 template <int D> __device__ __forceinline__ unsigned char* tile_of_slot(const RowsParams& p, int64_t slot, int head, int& tok) {
-    if (slot < 0 || slot >= p.num_slots) return nullptr;
     const int64_t page = slot / p.page_size;
     const int row = static_cast<int>(slot - page * p.page_size);
     tok = row & 15;
@@ -52,47 +86,74 @@ template <typename T> __device__ __forceinline__ float elt_round(float x);
 template <> __device__ __forceinline__ float elt_round<__nv_bfloat16>(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 template <> __device__ __forceinline__ float elt_round<__half>(float x) { return __half2float(__float2half_rn(x)); }
 
-// D / 8 threads per row (a row = one token, one head, K or V), 8 elements each.
+// The codes of 8 elements: low half dims 0, 2, 4, 6, high half 1, 3, 5, 7.
 //
-// scale = round16((max - lo) / 15), code = rint((x - lo) / scale) clipped to 15.  All quotients are IEEE
-// divisions of differences that are exact in fp32 unless the row spans more than 2^13: then every
-// code and scale is the one the definition gives in exact arithmetic.  A row with a NaN or an infinity is stored as
-// NaN scale and offset: whoever attends it sees it.
-template <typename T, int D> __global__ void __launch_bounds__(256) append_int4_kernel(const RowsParams p) {
-    constexpr int kLanes = D / 8;
-    const int64_t idx = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-    const int64_t r = idx / kLanes;
-    const int i = static_cast<int>(idx) % kLanes;
-    const bool have = r < p.num_rows;
-    const int per_token = 2 * p.heads;
-    const int64_t token = have ? r / per_token : 0;
-    const int rem = static_cast<int>(r - token * per_token);
-    const bool is_v = rem >= p.heads;
-    const int head = is_v ? rem - p.heads : rem;
-    int tok = 0;
-    unsigned char* tile = have ? tile_of_slot<D>(p, __ldg(p.slots + token), head, tok) : nullptr;
-
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (tile) {
-        const T* src = is_v ? static_cast<const T*>(p.value) + token * p.value_token + head * p.value_head
-                            : static_cast<const T*>(p.key) + token * p.key_token + head * p.key_head;
-        raw = __ldg(reinterpret_cast<const uint4*>(src) + i);
-    }
-    float x[8];
-    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 e = Int4Elt<T>::unpack(words[j]);
-        x[2 * j] = e.x;
-        x[2 * j + 1] = e.y;
-    }
-    float lo = x[0], hi = x[0];
-    bool bad = false;
+// code = rint((x - lo) / scale), halves to the even code, at most 15.  x - lo is exact in fp32 unless a row
+// spans more than 2^13 times its smallest step, so the quotient decides exactly; it costs an IEEE division only
+// where (x - lo) * (1 / scale), which is within 2^-18 of it, lies that near to a half.  Adding 1.5 * 2^23
+// rounds to an integer that then stands in the low mantissa bits.
+__device__ __forceinline__ uint32_t encode8(const float (&x)[8], float lo, float scale) {
+    constexpr float kMagic = 12582912.f;
+    constexpr uint32_t kMagicBits = 0x4B400000u;
+    const float inv = 1.f / scale;
+    uint32_t word = 0;
+    float worst = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        lo = fminf(lo, x[j]);
-        hi = fmaxf(hi, x[j]);
-        bad = bad || !(fabsf(x[j]) <= FLT_MAX);
+        const float t = fminf((x[j] - lo) * inv, 15.f);
+        const float u = t + kMagic;
+        worst = fmaxf(worst, fabsf(t - (u - kMagic)));
+        word += (__float_as_uint(u) - kMagicBits) << (4 * (j >> 1) + 16 * (j & 1));
+    }
+    if (worst > 0.5f - 4e-6f || !(inv < INFINITY)) {
+        word = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float t = fminf(rintf((x[j] - lo) / scale), 15.f);
+            word |= static_cast<uint32_t>(t) << (4 * (j >> 1) + 16 * (j & 1));
+        }
+    }
+    return word;
+}
+
+// D / 16 threads per row (one token, K or V), 16 elements each; the CTA's 32 rows in one or two passes.
+// A row with a NaN or an infinity is stored as NaN scale and offset: whoever attends it sees it.
+template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) append_int4_kernel(const RowsParams p) {
+    using L = Int4Tile<D>;
+    constexpr int kLanes = D / 16;
+    __shared__ __align__(16) unsigned char image[L::kBytes];
+    __shared__ TileGroup grp;
+    const int token0 = static_cast<int>(blockIdx.x / p.heads) * 16, head = blockIdx.x % p.heads;
+    const int row = threadIdx.x / kLanes, i = threadIdx.x % kLanes;
+    const int tok_in = row & 15;
+    const bool is_v = row >= 16;
+    // the rows are requested before the slots are looked at: a padding token's row is read for nothing
+    uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    const bool have = row < 32 && token0 + tok_in < p.num_tokens;
+    if (have) {
+        const int64_t token = token0 + tok_in;
+        const T* src = is_v ? static_cast<const T*>(p.value) + token * p.value_token + head * p.value_head
+                            : static_cast<const T*>(p.key) + token * p.key_token + head * p.key_head;
+        raw[0] = __ldg(reinterpret_cast<const uint4*>(src) + 2 * i);
+        raw[1] = __ldg(reinterpret_cast<const uint4*>(src) + 2 * i + 1);
+    }
+    load_group<D>(p, grp, token0, head);
+    float x[2][8];
+    const uint32_t words[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float2 e = Int4Elt<T>::unpack(words[j]);
+        x[j >> 2][2 * (j & 3)] = e.x;
+        x[j >> 2][2 * (j & 3) + 1] = e.y;
+    }
+    float lo = x[0][0], hi = x[0][0];
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float v = x[j >> 3][j & 7];
+        lo = fminf(lo, v);
+        hi = fmaxf(hi, v);
+        bad = bad || !(fabsf(v) <= FLT_MAX);
     }
 #pragma unroll
     for (int d = kLanes / 2; d > 0; d >>= 1) {
@@ -100,67 +161,97 @@ template <typename T, int D> __global__ void __launch_bounds__(256) append_int4_
         hi = fmaxf(hi, __shfl_xor_sync(kFullMask, hi, d));
     }
     const uint32_t bad_lanes = __ballot_sync(kFullMask, bad);
-    const int lane = threadIdx.x & 31;
-    bad = ((bad_lanes >> (lane & ~(kLanes - 1))) & ((1u << kLanes) - 1u)) != 0;
-    if (!tile) return;
-    // (a bf16 row may span more than fp32 can hold: then everything is halved, which is exact)
-    const float h = isinf(hi - lo) ? 0.5f : 1.f;
-    const float scale = bad ? NAN : elt_round<T>((h * hi - h * lo) / (15.f * h));
-    uint32_t word = 0;
-    if (scale > 0.f) {
+    bad = ((bad_lanes >> (threadIdx.x & 31 & ~(kLanes - 1))) & ((1u << kLanes) - 1u)) != 0;
+    float scale;
+    if (hi - lo <= FLT_MAX) {
+        scale = elt_round<T>((hi - lo) / 15.f);
+    } else {                   // a bf16 row may span more than fp32 can hold: everything halved, which is exact
+        scale = elt_round<T>((0.5f * hi - 0.5f * lo) / 7.5f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float t = fminf(rintf((h * x[j] - h * lo) / (h * scale)), 15.f);
-            // dims 0, 2, 4, 6 in the low half, 1, 3, 5, 7 in the high one
-            word |= static_cast<uint32_t>(t) << (4 * (j >> 1) + 16 * (j & 1));
+        for (int j = 0; j < 16; ++j) x[j >> 3][j & 7] *= 0.5f;
+    }
+    if (bad) scale = NAN;
+    const float half = hi - lo <= FLT_MAX ? 1.f : 0.5f;
+    const uint32_t prm = Elt<T>::pack(scale, bad ? NAN : lo);
+    uint32_t code[2] = {0, 0};
+    if (scale > 0.f) {
+        code[0] = encode8(x[0], half * lo, half * scale);
+        code[1] = encode8(x[1], half * lo, half * scale);
+    }
+    // where the row goes: the image of the tile, or straight to the cache
+    unsigned char* tile = image;
+    int tok = tok_in;
+    if (!grp.tile) {
+        const int64_t slot = grp.slot[tok_in];
+        tile = have && slot >= 0 ? tile_of_slot<D>(p, slot, head, tok) : nullptr;
+    }
+    if (tile && row < 32) {
+        if (!is_v) {
+            *reinterpret_cast<uint2*>(tile + k_word_off<D>(tok, 2 * i)) = make_uint2(code[0], code[1]);
+        } else {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint16_t* dst = reinterpret_cast<uint16_t*>(tile + v_half_off<D>(tok, 2 * i + b));
+                dst[0] = static_cast<uint16_t>(code[b]);
+                dst[2] = static_cast<uint16_t>(code[b] >> 16);
+            }
         }
+        if (i == 0) *reinterpret_cast<uint32_t*>(tile + (is_v ? L::kVPrm : L::kKPrm) + tok * 4) = prm;
     }
-    if (!is_v) {
-        *reinterpret_cast<uint32_t*>(tile + k_word_off<D>(tok, i)) = word;
-    } else {
-        uint16_t* dst = reinterpret_cast<uint16_t*>(tile + v_half_off<D>(tok, i));
-        dst[0] = static_cast<uint16_t>(word);
-        dst[2] = static_cast<uint16_t>(word >> 16);
+    if (grp.tile) {
+        __syncthreads();
+        for (int j = threadIdx.x; j < L::kBytes / 16; j += kRowThreads)
+            reinterpret_cast<uint4*>(grp.tile)[j] = reinterpret_cast<const uint4*>(image)[j];
     }
-    if (i == 0)
-        *reinterpret_cast<uint32_t*>(tile + (is_v ? Int4Tile<D>::kVPrm : Int4Tile<D>::kKPrm) + tok * 4) =
-            Elt<T>::pack(scale, bad ? NAN : lo);
 }
 
 // The inverse: value = lo + scale * code in fp32 (one rounding, the product is exact), rounded to T.
-template <typename T, int D> __global__ void __launch_bounds__(256) gather_int4_kernel(const RowsParams p) {
-    constexpr int kLanes = D / 8;
-    const int64_t idx = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-    const int64_t r = idx / kLanes;
-    const int i = static_cast<int>(idx) % kLanes;
-    if (r >= p.num_rows) return;
-    const int per_token = 2 * p.heads;
-    const int64_t token = r / per_token;
-    const int rem = static_cast<int>(r - token * per_token);
-    const bool is_v = rem >= p.heads;
-    const int head = is_v ? rem - p.heads : rem;
-    int tok = 0;
-    const unsigned char* tile = tile_of_slot<D>(p, __ldg(p.slots + token), head, tok);
-    if (!tile) return;
-    uint32_t word;
-    if (!is_v) {
-        word = *reinterpret_cast<const uint32_t*>(tile + k_word_off<D>(tok, i));
-    } else {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(tile + v_half_off<D>(tok, i));
-        word = src[0] | (static_cast<uint32_t>(src[2]) << 16);
+// D / 8 threads per row, 8 elements each.
+template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) gather_int4_kernel(const RowsParams p) {
+    using L = Int4Tile<D>;
+    constexpr int kLanes = D / 8, kRowsPerPass = kRowThreads / kLanes;
+    __shared__ __align__(16) unsigned char image[L::kBytes];
+    __shared__ TileGroup grp;
+    const int token0 = static_cast<int>(blockIdx.x / p.heads) * 16, head = blockIdx.x % p.heads;
+    load_group<D>(p, grp, token0, head);
+    if (grp.tile) {
+        for (int j = threadIdx.x; j < L::kBytes / 16; j += kRowThreads)
+            reinterpret_cast<uint4*>(image)[j] = __ldg(reinterpret_cast<const uint4*>(grp.tile) + j);
+        __syncthreads();
     }
-    const float2 prm = Int4Elt<T>::unpack(
-        *reinterpret_cast<const uint32_t*>(tile + (is_v ? Int4Tile<D>::kVPrm : Int4Tile<D>::kKPrm) + tok * 4));
-    uint32_t out[4];
+    const int i = threadIdx.x % kLanes;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float a = fmaf(static_cast<float>((word >> (4 * j)) & 15u), prm.x, prm.y);
-        const float b = fmaf(static_cast<float>((word >> (4 * j + 16)) & 15u), prm.x, prm.y);
-        out[j] = Elt<T>::pack(a, b);
+    for (int row = threadIdx.x / kLanes; row < 32; row += kRowsPerPass) {
+        const int tok_in = row & 15;
+        const bool is_v = row >= 16;
+        const unsigned char* tile = image;
+        int tok = tok_in;
+        if (!grp.tile) {
+            const int64_t slot = grp.slot[tok_in];
+            if (slot < 0) continue;
+            tile = tile_of_slot<D>(p, slot, head, tok);
+        }
+        uint32_t word;
+        if (!is_v) {
+            word = *reinterpret_cast<const uint32_t*>(tile + k_word_off<D>(tok, i));
+        } else {
+            const uint16_t* src = reinterpret_cast<const uint16_t*>(tile + v_half_off<D>(tok, i));
+            word = src[0] | (static_cast<uint32_t>(src[2]) << 16);
+        }
+        const float2 prm = Int4Elt<T>::unpack(*reinterpret_cast<const uint32_t*>(tile + (is_v ? L::kVPrm : L::kKPrm) + tok * 4));
+        const uint32_t pairs[4] = {Int4Elt<T>::template pair<0>(word), Int4Elt<T>::template pair<1>(word),
+                                   Int4Elt<T>::template pair<2>(word), Int4Elt<T>::template pair<3>(word)};
+        uint32_t out[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 c = Int4Elt<T>::unpack(pairs[j]);       // 16 + code
+            out[j] = Elt<T>::pack(fmaf(c.x - 16.f, prm.x, prm.y), fmaf(c.y - 16.f, prm.x, prm.y));
+        }
+        const int64_t token = token0 + tok_in;
+        T* dst = is_v ? static_cast<T*>(p.value) + token * p.value_token + head * p.value_head
+                      : static_cast<T*>(p.key) + token * p.key_token + head * p.key_head;
+        reinterpret_cast<uint4*>(dst)[i] = make_uint4(out[0], out[1], out[2], out[3]);
     }
-    T* dst = is_v ? static_cast<T*>(p.value) + token * p.value_token + head * p.value_head
-                  : static_cast<T*>(p.key) + token * p.key_token + head * p.key_head;
-    reinterpret_cast<uint4*>(dst)[i] = make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
@@ -177,6 +268,8 @@ int check_device(int* dev) {
     }
     return PAT_OK;
 }
+
+int64_t row_blocks(const pat_int4_rows_args& a) { return (static_cast<int64_t>(a.num_tokens) + 15) / 16 * a.num_kv_heads; }
 
 int rows_params(const pat_int4_rows_args& a, RowsParams* out) {
     if (a.num_tokens < 0 || a.num_kv_heads <= 0 || a.num_pages <= 0) return PAT_ERR_BAD_ARGUMENT;
@@ -202,11 +295,10 @@ int rows_params(const pat_int4_rows_args& a, RowsParams* out) {
     p.page_stride = a.page_stride;
     p.head_stride = a.head_stride;
     p.num_slots = a.num_pages * static_cast<int64_t>(a.page_size);
-    p.num_rows = static_cast<int64_t>(a.num_tokens) * 2 * a.num_kv_heads;
+    p.num_tokens = a.num_tokens;
     p.heads = a.num_kv_heads;
     p.page_size = a.page_size;
-    const int64_t blocks = (p.num_rows * (a.head_dim / 8) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return PAT_ERR_TOO_LARGE;
+    if (row_blocks(a) > 0x7fffffffLL || a.num_tokens > 0x7fffffff - 16) return PAT_ERR_TOO_LARGE;
     *out = p;
     return PAT_OK;
 }
@@ -292,8 +384,7 @@ int pat_b200_append_int4(const pat_int4_rows_args* args, void* stream_handle) {
     const bool bf16 = args->dtype == PAT_DTYPE_BF16;
     auto kern = args->head_dim == 128 ? (bf16 ? append_int4_kernel<__nv_bfloat16, 128> : append_int4_kernel<__half, 128>)
                                       : (bf16 ? append_int4_kernel<__nv_bfloat16, 64> : append_int4_kernel<__half, 64>);
-    const unsigned blocks = static_cast<unsigned>((p.num_rows * (args->head_dim / 8) + 255) / 256);
-    kern<<<blocks, 256, 0, static_cast<cudaStream_t>(stream_handle)>>>(p);
+    kern<<<static_cast<unsigned>(row_blocks(*args)), kRowThreads, 0, static_cast<cudaStream_t>(stream_handle)>>>(p);
     return cudaGetLastError() == cudaSuccess ? PAT_OK : PAT_ERR_CUDA;
 }
 
@@ -307,8 +398,7 @@ int pat_b200_gather_int4(const pat_int4_rows_args* args, void* stream_handle) {
     const bool bf16 = args->dtype == PAT_DTYPE_BF16;
     auto kern = args->head_dim == 128 ? (bf16 ? gather_int4_kernel<__nv_bfloat16, 128> : gather_int4_kernel<__half, 128>)
                                       : (bf16 ? gather_int4_kernel<__nv_bfloat16, 64> : gather_int4_kernel<__half, 64>);
-    const unsigned blocks = static_cast<unsigned>((p.num_rows * (args->head_dim / 8) + 255) / 256);
-    kern<<<blocks, 256, 0, static_cast<cudaStream_t>(stream_handle)>>>(p);
+    kern<<<static_cast<unsigned>(row_blocks(*args)), kRowThreads, 0, static_cast<cudaStream_t>(stream_handle)>>>(p);
     return cudaGetLastError() == cudaSuccess ? PAT_OK : PAT_ERR_CUDA;
 }
 

@@ -8,28 +8,30 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <vector>
 
 #include "../../include/pat_b200.h"
 
 namespace {
 
 constexpr int kMaxCaches = 64;         // tensors per launch
-constexpr int kMaxPairs = 256;         // host-planned pairs per launch
+constexpr int kFewPairs = 64;          // host-planned pairs per launch: the two sizes of the parameter block
+constexpr int kManyPairs = 2048;
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;             // 16-byte pieces in flight per thread
 
-struct CopyParams {
+template <int kCap> struct CopyParams {
     unsigned char* caches[kMaxCaches];
     const int64_t* device_pairs;       // [num_pairs][2], or null: `pairs`
     int64_t page_stride, row_stride;   // bytes
     int64_t num_pages;
     int32_t rows, row_vecs;            // a page = `rows` runs of row_vecs 16-byte pieces
     int32_t num_pairs, blocks_per_page;
-    int32_t pairs[kMaxPairs][2];
+    int32_t pairs[kCap][2];
 };
 
 // blockIdx.x = (pair * blocks_per_page + part), blockIdx.y = tensor.
-__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+template <int kCap> __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyParams<kCap> p) {
     const int pair = blockIdx.x / p.blocks_per_page, part = blockIdx.x - pair * p.blocks_per_page;
     int64_t from, to;
     if (p.device_pairs) {
@@ -61,6 +63,54 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
         if (first + i * kThreads < total) *reinterpret_cast<uint4*>(dst + off[i]) = v[i];
 }
 
+// No page may be the target of two pairs, nor a source and a target: the blocks run in any order.
+// One bit per page; the words that were set are cleared again, so the array stays zero between calls.
+int check_pairs(const int64_t* pairs, int64_t n, int64_t num_pages) {
+    static thread_local std::vector<uint64_t> marked;
+    for (int64_t i = 0; i < 2 * n; ++i)
+        if (pairs[i] < 0 || pairs[i] >= num_pages) return PAT_ERR_BAD_PLAN;
+    if (marked.size() < static_cast<size_t>(num_pages + 63) / 64) marked.resize(static_cast<size_t>(num_pages + 63) / 64, 0);
+    bool fine = true;
+    for (int64_t i = 0; i < n; ++i) {
+        uint64_t& w = marked[static_cast<size_t>(pairs[2 * i + 1]) >> 6];
+        const uint64_t bit = 1ull << (pairs[2 * i + 1] & 63);
+        fine = fine && !(w & bit);
+        w |= bit;
+    }
+    for (int64_t i = 0; i < n; ++i) fine = fine && !(marked[static_cast<size_t>(pairs[2 * i]) >> 6] >> (pairs[2 * i] & 63) & 1);
+    for (int64_t i = 0; i < n; ++i) marked[static_cast<size_t>(pairs[2 * i + 1]) >> 6] = 0;
+    return fine ? PAT_OK : PAT_ERR_BAD_PLAN;
+}
+
+template <int kCap> int launch_copies(const pat_copy_args& a, cudaStream_t stream) {
+    const int64_t vecs = static_cast<int64_t>(a.rows) * (a.row_bytes / 16);
+    CopyParams<kCap> p;
+    p.page_stride = a.page_stride;
+    p.row_stride = a.row_stride;
+    p.num_pages = a.num_pages;
+    p.rows = a.rows;
+    p.row_vecs = static_cast<int32_t>(a.row_bytes / 16);
+    p.blocks_per_page = static_cast<int32_t>((vecs + kThreads * kUnroll - 1) / (kThreads * kUnroll));
+    p.device_pairs = a.device_pairs;
+    const int chunk = a.host_pairs ? kCap : a.num_pairs;
+    if (static_cast<int64_t>(chunk < a.num_pairs ? chunk : a.num_pairs) * p.blocks_per_page > 0x7fffffffLL) return PAT_ERR_TOO_LARGE;
+    for (int c0 = 0; c0 < a.num_caches; c0 += kMaxCaches) {
+        const int nc = a.num_caches - c0 < kMaxCaches ? a.num_caches - c0 : kMaxCaches;
+        for (int i = 0; i < nc; ++i) p.caches[i] = static_cast<unsigned char*>(a.caches[c0 + i]);
+        for (int p0 = 0; p0 < a.num_pairs; p0 += chunk) {
+            const int np = a.num_pairs - p0 < chunk ? a.num_pairs - p0 : chunk;
+            if (a.host_pairs)
+                for (int i = 0; i < np; ++i) {
+                    p.pairs[i][0] = static_cast<int32_t>(a.host_pairs[2 * static_cast<int64_t>(p0 + i)]);
+                    p.pairs[i][1] = static_cast<int32_t>(a.host_pairs[2 * static_cast<int64_t>(p0 + i) + 1]);
+                }
+            copy_pages_kernel<kCap><<<dim3(static_cast<unsigned>(static_cast<int64_t>(np) * p.blocks_per_page), static_cast<unsigned>(nc)),
+                                      kThreads, 0, stream>>>(p);
+        }
+    }
+    return cudaGetLastError() == cudaSuccess ? PAT_OK : PAT_ERR_CUDA;
+}
+
 }  // namespace
 
 extern "C" int pat_b200_copy_pages(const pat_copy_args* args, void* stream_handle) {
@@ -71,38 +121,16 @@ extern "C" int pat_b200_copy_pages(const pat_copy_args* args, void* stream_handl
     if (!a.caches || (!a.host_pairs && !a.device_pairs) || (a.host_pairs && a.device_pairs)) return PAT_ERR_BAD_ARGUMENT;
     if (a.row_bytes % 16 != 0 || a.row_stride % 16 != 0 || a.page_stride % 16 != 0 || a.page_stride <= 0) return PAT_ERR_UNSUPPORTED;
     if (a.rows > 1 && a.row_stride < a.row_bytes) return PAT_ERR_UNSUPPORTED;
-    const int64_t vecs = static_cast<int64_t>(a.rows) * (a.row_bytes / 16);
-    if (vecs > 0x7fffffffLL - kThreads * kUnroll) return PAT_ERR_TOO_LARGE;
+    if (static_cast<int64_t>(a.rows) * (a.row_bytes / 16) > 0x7fffffffLL - kThreads * kUnroll || a.num_pages > 0x7fffffffLL)
+        return PAT_ERR_TOO_LARGE;
     for (int i = 0; i < a.num_caches; ++i)
         if (!a.caches[i] || (reinterpret_cast<uintptr_t>(a.caches[i]) & 15)) return PAT_ERR_UNSUPPORTED;
-    if (a.host_pairs)
-        for (int64_t i = 0; i < 2 * static_cast<int64_t>(a.num_pairs); ++i)
-            if (a.host_pairs[i] < 0 || a.host_pairs[i] >= a.num_pages) return PAT_ERR_BAD_PLAN;
-    CopyParams p;
-    p.page_stride = a.page_stride;
-    p.row_stride = a.row_stride;
-    p.num_pages = a.num_pages;
-    p.rows = a.rows;
-    p.row_vecs = static_cast<int32_t>(a.row_bytes / 16);
-    p.blocks_per_page = static_cast<int32_t>((vecs + kThreads * kUnroll - 1) / (kThreads * kUnroll));
-    const int chunk = a.host_pairs ? kMaxPairs : a.num_pairs;
-    for (int c0 = 0; c0 < a.num_caches; c0 += kMaxCaches) {
-        const int nc = a.num_caches - c0 < kMaxCaches ? a.num_caches - c0 : kMaxCaches;
-        for (int i = 0; i < nc; ++i) p.caches[i] = static_cast<unsigned char*>(a.caches[c0 + i]);
-        for (int p0 = 0; p0 < a.num_pairs; p0 += chunk) {
-            const int np = a.num_pairs - p0 < chunk ? a.num_pairs - p0 : chunk;
-            p.num_pairs = np;
-            p.device_pairs = a.device_pairs;
-            if (a.host_pairs)
-                for (int i = 0; i < np; ++i) {
-                    p.pairs[i][0] = static_cast<int32_t>(a.host_pairs[2 * (p0 + i)]);
-                    p.pairs[i][1] = static_cast<int32_t>(a.host_pairs[2 * (p0 + i) + 1]);
-                }
-            const int64_t blocks = static_cast<int64_t>(np) * p.blocks_per_page;
-            if (blocks > 0x7fffffffLL) return PAT_ERR_TOO_LARGE;
-            copy_pages_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(nc)), kThreads, 0,
-                                static_cast<cudaStream_t>(stream_handle)>>>(p);
-        }
+    if (a.host_pairs) {
+        try {
+            const int rc = check_pairs(a.host_pairs, a.num_pairs, a.num_pages);
+            if (rc != PAT_OK) return rc;
+        } catch (...) { return PAT_ERR_NO_MEMORY; }
     }
-    return cudaGetLastError() == cudaSuccess ? PAT_OK : PAT_ERR_CUDA;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+    return a.num_pairs <= kFewPairs || a.device_pairs ? launch_copies<kFewPairs>(a, stream) : launch_copies<kManyPairs>(a, stream);
 }
