@@ -129,7 +129,8 @@ typedef struct pat_work_options {
     int32_t grow_slack_pages;    /* lists built from a tree: free page slots kept behind the page list of
                                     every request's own last segment, so that pat_work_advance can append
                                     pages in place.  0 = default (8), < 0 = none */
-    int32_t reserved;
+    int32_t stream_rows;         /* query rows per streaming item, at least the head ratio, at most 16; 0 = 16.
+                                    pat_b200_decode_int4 runs 8 at a time */
 } pat_work_options;
 
 typedef struct pat_work_header {

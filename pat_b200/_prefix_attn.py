@@ -29,7 +29,8 @@ class WorkConfig:
     """Tuning knobs of the work-list builder (0 = library default)."""
 
     __slots__ = ("num_sms", "dense_min_rows", "chunk_tokens_min", "chunk_tokens_max",
-                 "dense_piece_tokens_min", "items_per_sm", "disable_dense", "dense_tile_ns", "grow_slack_pages")
+                 "dense_piece_tokens_min", "items_per_sm", "disable_dense", "dense_tile_ns", "grow_slack_pages",
+                 "stream_rows")
 
     def __init__(self, **kw):
         for name in self.__slots__:
@@ -77,7 +78,10 @@ def set_default_config(cfg: Optional[WorkConfig]) -> None:
 def int4_config() -> WorkConfig:
     """Options of the work lists for a 4-bit cache."""
     cfg = WorkConfig(**{n: getattr(default_config(), n) for n in WorkConfig.__slots__})
-    cfg.disable_dense = 1
+    cfg.stream_rows = cfg.stream_rows or 8
+    cfg.items_per_sm = cfg.items_per_sm or 16
+    cfg.chunk_tokens_min = cfg.chunk_tokens_min or 128
+    cfg.dense_tile_ns = cfg.dense_tile_ns or -1
     return cfg
 
 

@@ -35,6 +35,7 @@ pat::WorkOptions to_options(const pat_work_options* o) {
     if (o->dense_tile_ns != 0) w.dense_tile_ns = o->dense_tile_ns;
     if (o->grow_slack_pages > 0) w.grow_slack_pages = o->grow_slack_pages;
     if (o->grow_slack_pages < 0) w.grow_slack_pages = 0;
+    if (o->stream_rows > 0 && o->stream_rows < w.stream_rows) w.stream_rows = o->stream_rows;
     if (o->disable_dense) { w.dense_rows = 0; w.dense_min_rows = 1 << 30; }
     return w;
 }

@@ -144,7 +144,7 @@ int launch_all(const pat_decode_args& a, cudaStream_t stream, int dev) {
         // shared segments on tcgen05 / TMEM: persistent CTAs, one per share of the dense work
         static std::atomic<bool> configured[kMaxDevices][2];    // zero-initialised; set once per device
         auto kern = limits ? dense_tc_kernel<T, D, true> : dense_tc_kernel<T, D, false>;
-        constexpr int smem = TcSmem<D>::kRequest;
+        constexpr int smem = TcSmem<D, false>::kRequest;
         if (!configured[dev][limits].load(std::memory_order_acquire)) {
             if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
                 return PAT_ERR_CUDA;

@@ -39,6 +39,7 @@
 // before the CTA frees its TMEM and returns.
 #pragma once
 
+#include "pat_int4.cuh"
 #include "pat_kernels.cuh"
 
 namespace pat {
@@ -47,19 +48,34 @@ constexpr int kTcTile = 128;                // tokens per tile
 constexpr int kTcRing = 3;                  // depth of the K, V and S rings
 constexpr int kTcSoftmaxWarps = 8;
 constexpr int kTcThreads = (kTcSoftmaxWarps + 3) * 32;
+// 4-bit cache: warp 8 requests the raw tiles, warps 10-15 unpack.  Sixteen warps start with 128 registers a thread (the register file);
+// the unpacking warpgroups hand 40 of them each to the softmax warpgroups.
+constexpr int kTcUnpackK = 2, kTcUnpackV = 4;       // warps per operand: V takes twice the arithmetic
+constexpr int kTcUnpackWarps = kTcUnpackK + kTcUnpackV;
+constexpr int kTcInt4Threads = (kTcSoftmaxWarps + 2 + kTcUnpackWarps) * 32;
+constexpr int kTcSoftmaxRegs = 168, kTcUnpackRegs = 88;
+static_assert(kTcSoftmaxWarps * kTcSoftmaxRegs + (2 + kTcUnpackWarps) * kTcUnpackRegs <= 16 * 128 && kTcInt4Threads == 512,
+              "the split must fit what the block was launched with");
 constexpr int kTcTmemCols = 512;
 constexpr float kTcLazyLog2 = 8.0f;
 
-template <int D> struct TcSmem {
+// kInt4: the cache holds 4-bit codes (pat_int4.cuh).  Raw tiles arrive in granules of 64 tokens (half a tile), in a
+// ring of their own that covers the way from memory; the unpacked tiles then need two slots each.
+template <int D, bool kInt4> struct TcSmem {
     static constexpr int kBoxes = D / 64;
+    static constexpr int kKvRing = kInt4 ? 2 : kTcRing;
+    static constexpr int kPrmRing = 4, kRawRing = 7;
+    static constexpr int kRawBytes = 4 * Int4Tile<D>::kBytes;
     static constexpr int kQBytes = kBoxes * 128 * 128;          // [box][128 rows][128 B]
     static constexpr int kKBytes = kBoxes * kTcTile * 128;      // [box][128 tokens][128 B]
     static constexpr int kQOff = 0;
     static constexpr int kKOff = kQOff + kQBytes;               // K ring
-    static constexpr int kVOff = kKOff + kTcRing * kKBytes;     // V ring
-    static constexpr int kBarOff = kVOff + kTcRing * kKBytes;   // 43 mbarriers + tmem base word + flag
+    static constexpr int kVOff = kKOff + kKvRing * kKBytes;     // V ring
+    static constexpr int kRawOff = kVOff + kKvRing * kKBytes;
+    static constexpr int kBarOff = kRawOff + (kInt4 ? kRawRing * kRawBytes : 0);    // 43 mbarriers (kInt4: 61) + tmem base word + flag
     static constexpr int kXchOff = kBarOff + 512;               // float[2][2][128]: row maxima / sums of the two column halves
-    static constexpr int kRequest = kXchOff + 2048;
+    static constexpr int kPrmOff = kXchOff + 2048;              // kInt4: float[ring][2][128], factor and addend of every token's scores
+    static constexpr int kRequest = kPrmOff + (kInt4 ? kPrmRing * 1024 : 0);
 };
 
 // ---- tcgen05 wrappers ------------------------------------------------------------
@@ -169,6 +185,24 @@ template <typename T> __device__ __forceinline__ uint32_t umma_idesc(int m, int 
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 __device__ __forceinline__ void named_bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -210,15 +244,265 @@ struct DenseTcParams {
 };
 
 // ------------------------------------------------------------------------------------
+// 4-bit cache: the warps that turn raw tiles into the 16-bit K and V tiles of the MMAs.
+//
+// K: the codes go to the tensor cores as they are (16 + c, exact), and the softmax warps turn a product into a
+// score with the token's scale and offset in fp32:  x = (s (q . (16 + c)) + (lo - 16 s) sum(q)) * scale * log2 e.
+// (Rounded K values would put 2^-9 of noise into every bf16 score and through it into the LSE.)  V: values in
+// the model's type, v = lo + s c in one fma of the exact code, rounded once - half a step, like P beside it.
+// A token past the item's end becomes zeros.  One whose V row is NaN gets zeros for V and NaN scores: whoever sees
+// it returns NaN, and for rows that must not see it (kLimits) 0 * V stays 0.
+//
+// Two codes to two 16-bit floats 16 + c cost a shift and a logic instruction, a V value pair a subtraction
+// and an fma more.  Lanes own what the cache layout makes whole words, and pairs of lanes take the chunks of
+// their rows in different order so that eight lanes' 16-byte stores fall into eight different bank groups of the
+// swizzled rows.
+template <typename T> struct Pack2;
+template <> struct Pack2<__nv_bfloat16> {
+    using V = __nv_bfloat162;
+    static constexpr uint32_t kExp = 0x7f80u;
+};
+template <> struct Pack2<__half> {
+    using V = __half2;
+    static constexpr uint32_t kExp = 0x7c00u;
+};
+template <typename T> __device__ __forceinline__ uint32_t code_pair_value(uint32_t sixteen_plus_c, uint32_t ss, uint32_t ll) {
+    using V = typename Pack2<T>::V;
+    const uint32_t k16 = Int4Elt<T>::kSixteen;
+    const V c = __hsub2(*reinterpret_cast<const V*>(&sixteen_plus_c), *reinterpret_cast<const V*>(&k16));
+    const V v = __hfma2(c, *reinterpret_cast<const V*>(&ss), *reinterpret_cast<const V*>(&ll));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// 8 codes of one word (nibble j of the low half: element 2j, of the high half: 2j + 1) -> 16 bytes at `dst`
+template <typename T> __device__ __forceinline__ void store_codes(uint32_t dst, uint32_t word) {
+    using E = Int4Elt<T>;
+    // (no memory clobber: the loads of the next words may pass; the fence before the arrival orders the stores)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(E::template pair<0>(word)),
+                 "r"(E::template pair<1>(word)), "r"(E::template pair<2>(word)), "r"(E::template pair<3>(word)));
+}
+template <typename T> __device__ __forceinline__ void store_values(uint32_t dst, uint32_t word, uint32_t ss, uint32_t ll) {
+    using E = Int4Elt<T>;
+    const uint32_t a = code_pair_value<T>(E::template pair<0>(word), ss, ll), b = code_pair_value<T>(E::template pair<1>(word), ss, ll);
+    const uint32_t c = code_pair_value<T>(E::template pair<2>(word), ss, ll), d = code_pair_value<T>(E::template pair<3>(word), ss, ll);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d));
+}
+// scale and offset of a token, each doubled to a pair
+__device__ __forceinline__ void split_params(uint32_t prm, uint32_t& ss, uint32_t& ll) {
+    ss = __byte_perm(prm, prm, 0x1010);
+    ll = __byte_perm(prm, prm, 0x3232);
+}
+template <typename T> __device__ __forceinline__ bool params_are_finite(uint32_t prm) {
+    constexpr uint32_t e = Pack2<T>::kExp;
+    return (prm & e) != e && (prm >> 16 & e) != e;
+}
+
+// The warp that requests the raw granules.  Page ids are fetched a granule ahead of the request that needs them.
+template <typename T, int D>
+__device__ __forceinline__ void load_granules(const DenseTcParams& dp, const Int4Cache& cache, int lane, int item_lo, int item_hi,
+                                              uint32_t raw, uint32_t bar_raw) {
+    using L = TcSmem<D, true>;
+    using I = Int4Tile<D>;
+    constexpr int RR = L::kRawRing;
+    const AttnParams& p = dp.a;
+    const uint32_t raw_full = bar_raw, raw_empty = bar_raw + 8 * RR;
+    const int tiles_per_page = p.page_size >> 4;
+    int item = item_lo, sub = 0;            // granule under the cursor
+    int subs = 0, page = 0, in_page = 0, kvh = 0;
+    auto look_up = [&]() {                  // fetches its page ids and moves on
+        subs = 0;
+        if (item >= item_hi) return;
+        const int32_t* it = p.items + static_cast<size_t>(item) * 8;
+        const int page_off = __ldg(it + 2), subs_all = (__ldg(it + 3) + 15) >> 4;
+        kvh = __ldg(it + 5);
+        subs = min(4, subs_all - sub);
+        const int st = sub + lane, at = st / tiles_per_page;
+        in_page = st - at * tiles_per_page;
+        page = lane < subs ? __ldg(p.pages + page_off + at) : 0;
+        if ((sub += 4) < subs_all) return;
+        ++item;
+        sub = 0;
+        if (item < item_hi) {
+            // pull the next item's record, query ids and Q rows (scattered by query id) towards this SM: the
+            // softmax warps fetch them between two tiles
+            const int4* nx = reinterpret_cast<const int4*>(p.items + static_cast<size_t>(item) * 8);
+            const int n_rows = __ldg(nx).y * p.hratio, n_kvh = __ldg(nx + 1).y;
+            const int32_t* ids = dp.dense_q + static_cast<size_t>(item) * dp.dense_q_width;
+            for (int row = lane; row < n_rows; row += 32) {
+                const int qi = row / p.hratio, gg = row - qi * p.hratio;
+                const T* q = q_row_ptr<T>(p, __ldg(ids + qi), n_kvh * p.hratio + gg);
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+                if constexpr (D * sizeof(T) > 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64));
+            }
+            __syncwarp();
+        }
+    };
+    bool ok = true;
+    int n = 0, slot = 0;
+    uint32_t phase = 1;                     // parity of the release that precedes the current use of the slot
+    look_up();
+    while (subs > 0) {
+        const int now = subs, now_in_page = in_page, now_kvh = kvh;
+        const int64_t now_page = page;
+        look_up();                          // in flight while this one waits for its slot
+        if (n >= RR) ok = __all_sync(kFullMask, mbar_wait_in<true>(raw_empty + 8 * slot, phase, p.wait_ns));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(raw_full + 8 * slot, now * I::kBytes);
+        __syncwarp();
+        if (lane < now)
+            bulk_load(raw + slot * L::kRawBytes + lane * I::kBytes,
+                      cache.base + now_page * cache.page_stride + now_kvh * cache.head_stride + now_in_page * I::kBytes, I::kBytes,
+                      raw_full + 8 * slot);
+        ++n;
+        if (++slot == RR) { slot = 0; phase ^= 1; }
+    }
+    if (!ok) {
+        // Gave up: nothing more is requested; granules still on their way get a short second wait so that none lands
+        // after the CTA has handed its shared memory back.
+        if (lane == 0 && p.status) atomicExch(p.status, 11);
+        for (int i = max(0, n - RR); i < n; ++i) mbar_wait_in<true>(raw_full + 8 * (i % RR), (i / RR) & 1, kDrainWaitNs);
+    }
+}
+
+// One warp of the K group (kV = false) or of the V group; the four 16-token groups of a granule are dealt out to the
+// warps of a group.
+template <typename T, int D, bool kV>
+__device__ __forceinline__ void unpack_operand(const DenseTcParams& dp, int who, int lane, int item_lo, int item_hi, uint32_t ring,
+                                               const unsigned char* raw, uint32_t bar_full, uint32_t bar_empty, uint32_t bar_raw,
+                                               float* prm, uint32_t bar_prm) {
+    using L = TcSmem<D, true>;
+    using I = Int4Tile<D>;
+    constexpr int kWords = D / 32, kGroup = kV ? kTcUnpackV : kTcUnpackK, kRing = L::kKvRing, RR = L::kRawRing;
+    const AttnParams& p = dp.a;
+    const int g = lane >> 2, c = lane & 3;
+    const uint32_t raw_full = bar_raw, raw_empty = bar_raw + 8 * RR;
+    bool ok = true;
+    // Where this lane's words go inside a row, K: word i is chunk (D/32) c + i of token g (+ 8), 8 chunks per
+    // 64-element box; D = 128: lanes 2, 3 of a row write to the second box at the same banks, so they take the words in
+    // another order.  V: chunk i of two of this lane's tokens, odd g the other way round.  The rows' swizzle (row & 7)
+    // is the same in every unit.
+    uint32_t place[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+        if constexpr (!kV) {
+            const int chunk = kWords * c + (D == 128 ? i ^ (c & 2) : i);
+            place[i] = (chunk >> 3) * (kTcTile * 128) + swz128(g, chunk & 7);
+        } else {
+            const int e = i / (kWords / 2), k = i % (kWords / 2);        // token of the pair, chunk
+            const int chunk = (kWords / 2) * g + (D == 128 ? k ^ (g & 1) : k);
+            place[i] = (chunk >> 3) * (kTcTile * 128) + swz128(2 * c + e, chunk & 7);
+        }
+    }
+    int t = 0, slot = 0, rs = 0;
+    uint32_t free_phase = 1, raw_phase = 0;     // parity of the release that precedes the current use of the slot; of granule rs
+    for (int item = item_lo; item < item_hi && ok; ++item) {
+        const int kv_len = __ldg(p.items + static_cast<size_t>(item) * 8 + 3);
+        for (int tok0 = 0; tok0 < kv_len; tok0 += kTcTile, ++t) {
+            const int valid = min(kTcTile, kv_len - tok0);
+            if (t >= kRing) ok = __all_sync(kFullMask, mbar_wait_in<true>(bar_empty + 8 * slot, free_phase, p.wait_ns));
+            if (!ok) break;
+            const uint32_t base = ring + slot * L::kKBytes;
+            // (None of the loops is unrolled: the roles of this kernel share the SM's instruction cache, and unrolled
+            // the tile took twice as long.)
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                const bool loaded = half * 64 < valid;          // else the half is past the item's end: zeros
+                if (loaded && ok) ok = __all_sync(kFullMask, mbar_wait_in<true>(raw_full + 8 * rs, raw_phase, p.wait_ns));
+                if (!ok) break;
+                const unsigned char* rt = raw + rs * L::kRawBytes;
+                if (!kV && who == 0) {          // two tokens a lane: what turns their products into scores
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int tok = lane + 32 * e, row = half * 64 + tok;
+                        const unsigned char* src = rt + (tok >> 4) * I::kBytes + (tok & 15) * 4;
+                        float factor = 0.f, addend = 0.f;
+                        if (row < valid) {
+                            const float2 kp = Int4Elt<T>::unpack(*reinterpret_cast<const uint32_t*>(src + I::kKPrm));
+                            factor = kp.x * p.scale_log2;
+                            addend = params_are_finite<T>(*reinterpret_cast<const uint32_t*>(src + I::kVPrm))
+                                         ? (kp.y - 16.f * kp.x) * p.scale_log2 : NAN;
+                        }
+                        prm[(t & 3) * 256 + row] = factor;
+                        prm[(t & 3) * 256 + 128 + row] = addend;
+                    }
+                }
+#pragma unroll 1
+                for (int u = who; u < 4; u += kGroup) {         // 16 tokens, as two units whose arithmetic interleaves
+                    const unsigned char* src = rt + u * I::kBytes;
+                    const uint32_t row0 = half * 64 + u * 16, dst = base + row0 * 128;
+                    uint32_t w[2][kWords];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < kWords; ++i) w[h][i] = 0;
+                    if constexpr (!kV) {
+                        if (loaded) {
+                            lds_words(w[0], src + g * I::kTokenBytes + c * (D / 8));
+                            lds_words(w[1], src + (g + 8) * I::kTokenBytes + c * (D / 8));
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < kWords; ++i)
+                                store_codes<T>(dst + h * 1024 + place[i], D == 128 && (c & 2) ? w[h][i ^ 2] : w[h][i]);
+                    } else {
+                        uint2 prm2[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+                        if (loaded) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                lds_words(w[h], src + I::kVOff + h * 4 * D + lane * I::kLaneBytes);
+                                prm2[h] = *reinterpret_cast<const uint2*>(src + I::kVPrm + (2 * c + 8 * h) * 4);
+                            }
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t vp = e == 0 ? prm2[h].x : prm2[h].y;
+                                const bool keep = static_cast<int>(row0) + 2 * c + 8 * h + e < valid && params_are_finite<T>(vp);
+                                uint32_t ss, ll, y[kWords / 2];      // words of 8 consecutive dims of this token
+                                split_params(keep ? vp : 0u, ss, ll);
+#pragma unroll
+                                for (int i = 0; i < kWords / 2; ++i)
+                                    y[i] = __byte_perm(w[h][2 * i], w[h][2 * i + 1], e == 0 ? 0x5410 : 0x7632);
+#pragma unroll
+                                for (int i = 0; i < kWords / 2; ++i)
+                                    store_values<T>(dst + h * 1024 + place[e * (kWords / 2) + i],
+                                                    D == 128 && (g & 1) ? y[i ^ 1] : y[i], ss, ll);
+                            }
+                    }
+                }
+                if (loaded) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(raw_empty + 8 * rs);
+                    if (++rs == RR) { rs = 0; raw_phase ^= 1; }
+                }
+            }
+            if (!ok) break;
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(bar_full + 8 * slot);
+                // (The next use of a parameter slot, four tiles on, waits for the product of tile t + 2, which is
+                // requested after the P V of tile t and so after that tile's softmax.)
+                if (!kV) mbar_arrive(bar_prm + 8 * (t & 3));
+            }
+            if (++slot == kRing) { slot = 0; free_phase ^= 1; }
+        }
+    }
+    if (!ok && lane == 0 && p.status) atomicExch(p.status, 11);
+}
+
+// ------------------------------------------------------------------------------------
 // kLimits: several query positions per request; a row may then see only the first part of an
 // item's tokens (AttnParams::limits), down to none of them.
-template <typename T, int D, bool kLimits>
-__global__ void __launch_bounds__(kTcThreads, 1)
-dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+// kInt4: the K and V tiles are unpacked from a 4-bit cache (`cache`) instead of loaded by TMA (kmap, vmap).
+template <typename T, int D, bool kLimits, bool kInt4>
+__device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                                              const Int4Cache& cache) {
     // This CTA is running: a kernel launched as this one's programmatic dependent (the streaming
     // kernel, which does not use this kernel's results) may start once every CTA has said so.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    using L = TcSmem<D>;
+    using L = TcSmem<D, kInt4>;
     constexpr int R = kTcRing;
     constexpr int kSW = kTcSoftmaxWarps;        // warps 0..7 softmax, 8 = K producer, 9 = MMA, 10 = V producer
     const AttnParams& p = dp.a;
@@ -244,7 +528,7 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
         return;
     }
     const uint32_t sQ = base + L::kQOff, sK = base + L::kKOff, sV = base + L::kVOff;
-    const uint32_t bars = base + L::kBarOff;
+    const uint32_t bars = base + L::kBarOff, sRaw = base + L::kRawOff;
     // barrier map (8 bytes each): full_k[R] empty_k[R] full_v[R] empty_v[R] s_full[R] p_ready[R]
     // o_done[R] q_ready o_free drain
     const uint32_t bar_full_k = bars, bar_empty_k = bars + 8 * R, bar_full_v = bars + 16 * R, bar_empty_v = bars + 24 * R,
@@ -252,6 +536,7 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
                    bar_ofree = bars + 56 * R + 8, bar_drain = bars + 56 * R + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tc_smem + L::kBarOff + 56 * R + 24);
     volatile int* poisoned = reinterpret_cast<volatile int*>(tc_smem + L::kBarOff + 56 * R + 32);
+    const uint32_t bar_prm = bars + 56 * R + 40, bar_raw = bar_prm + 32;        // kInt4: [4]; full [7], empty [7]
     float* xch = reinterpret_cast<float*>(tc_smem + L::kXchOff);      // [2][2][128]
 
     // If an earlier CTA of this call already gave up on a wait, do not start (uniform decision).
@@ -264,9 +549,15 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
     }
 
     if (tid == 0) {
-        tma_prefetch_desc(&kmap);
-        tma_prefetch_desc(&vmap);
-        for (int i = 0; i < 5 * R; ++i) mbar_init(bar_full_k + 8 * i, 1);       // full/empty k/v, s_full
+        if constexpr (!kInt4) {
+            tma_prefetch_desc(kmap);
+            tma_prefetch_desc(vmap);
+        }
+        for (int i = 0; i < 5 * R; ++i)                                         // full/empty k/v, s_full
+            mbar_init(bar_full_k + 8 * i, !kInt4 ? 1 : i / R == 0 ? kTcUnpackK : i / R == 2 ? kTcUnpackV : 1);
+        if constexpr (kInt4)
+            for (int i = 0; i < L::kPrmRing + 2 * L::kRawRing; ++i)
+                mbar_init(bar_prm + 8 * i, i < L::kPrmRing ? kTcUnpackK : i < L::kPrmRing + L::kRawRing ? 1 : kTcUnpackWarps);
         for (int i = 0; i < R; ++i) mbar_init(bar_p + 8 * i, kSW * 32);         // p_ready: every softmax thread
         for (int i = 0; i < R; ++i) mbar_init(bar_o + 8 * i, 1);                // o_done
         mbar_init(bar_q, kSW * 32);                                             // q_ready
@@ -282,10 +573,25 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
     const uint32_t tmem_o_col = R * kTcTile;    // O behind the S ring
     const int tiles_per_page = p.page_size >> 4;
 
-    if (warp == kSW || warp == kSW + 2) {
+    if (warp >= kSW) {
+    if constexpr (kInt4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcUnpackRegs));
+    if (kInt4 && warp != kSW + 1) {
+        if constexpr (kInt4) {
+            const int who = warp - kSW - 2;                         // K warps, then V warps
+            float* prm = reinterpret_cast<float*>(tc_smem + L::kPrmOff);
+            if (warp == kSW)
+                load_granules<T, D>(dp, cache, lane, item_lo, item_hi, sRaw, bar_raw);
+            else if (who < kTcUnpackK)
+                unpack_operand<T, D, false>(dp, who, lane, item_lo, item_hi, sK, tc_smem + L::kRawOff, bar_full_k, bar_empty_k,
+                                             bar_raw, prm, bar_prm);
+            else
+                unpack_operand<T, D, true>(dp, who - kTcUnpackK, lane, item_lo, item_hi, sV, tc_smem + L::kRawOff, bar_full_v,
+                                            bar_empty_v, bar_raw, prm, bar_prm);
+        }
+    } else if (!kInt4 && warp != kSW + 1) {
         // ---- TMA producers: one warp streams K, one streams V ---------------------------------
         const bool is_k = warp == kSW;
-        const CUtensorMap* map = is_k ? &kmap : &vmap;
+        const CUtensorMap* map = is_k ? kmap : vmap;
         const uint32_t ring = is_k ? sK : sV;
         const uint32_t full = is_k ? bar_full_k : bar_full_v;
         const uint32_t empty = is_k ? bar_empty_k : bar_empty_v;
@@ -317,7 +623,7 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
             }
             __syncwarp();
             for (int j = 0; j < n_tiles; ++j, ++t) {
-                if (t >= R) ok = mbar_wait(empty + 8 * s, ph, p.wait_ns);
+                if (t >= R) ok = mbar_wait_in<kInt4>(empty + 8 * s, ph, p.wait_ns);
                 if (!ok) break;
                 constexpr int kSub = kTcTile / 16;
                 const int subs = min(kSub, n_sub - j * kSub);
@@ -341,9 +647,9 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
             // way into the ring; give each a short second wait so that none lands after the CTA
             // has handed its shared memory back.
             if (lane == 0 && p.status) atomicExch(p.status, 11);
-            for (int tt = max(0, t - R); tt < t; ++tt) mbar_wait(full + 8 * (tt % R), (tt / R) & 1, kDrainWaitNs);
+            for (int tt = max(0, t - R); tt < t; ++tt) mbar_wait_in<kInt4>(full + 8 * (tt % R), (tt / R) & 1, kDrainWaitNs);
         }
-    } else if (warp == kSW + 1) {
+    } else {
         // ---- MMA issuer (one thread) -------------------------------------------------------------
         // The issuing thread is the narrowest resource of the CTA, so every descriptor is reduced
         // to "base word + slot * stride + constant": the high words are constants, the low words
@@ -390,17 +696,18 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
                 const bool opens = qk_j == 0;
                 if (opens && qk_tile > pv_done + 1) break;
                 const int slot = qk_tile % R;
-                const uint32_t phase = static_cast<uint32_t>(qk_tile / R) & 1u;
+                const int kslot = kInt4 ? qk_tile & 1 : slot;       // slot of the K ring
+                const uint32_t phase = static_cast<uint32_t>(kInt4 ? qk_tile >> 1 : qk_tile / R) & 1u;
                 if (opens) {
-                    ok = mbar_wait(bar_q, qk_items & 1, p.wait_ns);
+                    ok = mbar_wait_in<kInt4>(bar_q, qk_items & 1, p.wait_ns);
                     ++qk_items;
                     fence_async_smem();     // the Q rows were written through the generic proxy
                 }
-                if (ok) ok = mbar_wait(bar_full_k + 8 * slot, phase, p.wait_ns);
+                if (ok) ok = mbar_wait_in<kInt4>(bar_full_k + 8 * kslot, phase, p.wait_ns);
                 ok = __all_sync(kFullMask, ok);
                 if (!ok) return;            // gave up: nothing more is issued
                 tc_fence_after();
-                uint32_t q_w = q_lo, k_w = k_lo0 + slot * kSlotStep, acc = 0;
+                uint32_t q_w = q_lo, k_w = k_lo0 + kslot * kSlotStep, acc = 0;
 #pragma unroll
                 for (int ks = 0; ks < kSteps; ++ks) {
                     if (elect_one()) tc_mma(tmem_base + slot * kTcTile, desc(q_w), desc(k_w), idesc_qk, acc);
@@ -411,7 +718,7 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
                     acc = 1;
                 }
                 if (elect_one()) tc_commit(bar_s + 8 * slot);
-                if (elect_one()) tc_commit(bar_empty_k + 8 * slot);    // the K tile is free once this product has completed
+                if (elect_one()) tc_commit(bar_empty_k + 8 * kslot);    // the K tile is free once this product has completed
                 if (++qk_j == qk_n) { ++qk_item; qk_j = 0; qk_n = tiles_of(qk_item); }
                 ++qk_tile;
             }
@@ -421,15 +728,16 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
         issue_qk_upto(-1);
         for (int g = 0; g < total_tiles && ok; ++g) {
             // O += P(g) V(g)
-            ok = mbar_wait(bar_full_v + 8 * s, ph, p.wait_ns);
-            if (ok) ok = mbar_wait(bar_p + 8 * s, ph, p.wait_ns);  // P(g) is in TMEM (over S(g))
+            const int vslot = kInt4 ? g & 1 : s;                    // slot of the V ring
+            ok = mbar_wait_in<kInt4>(bar_full_v + 8 * vslot, kInt4 ? static_cast<uint32_t>(g >> 1) & 1u : ph, p.wait_ns);
+            if (ok) ok = mbar_wait_in<kInt4>(bar_p + 8 * s, ph, p.wait_ns);  // P(g) is in TMEM (over S(g))
             if (pv_j == 0 && pv_items > 0 && ok)
-                ok = mbar_wait(bar_ofree, (pv_items - 1) & 1, p.wait_ns);   // the softmax warps have read the previous item's O
+                ok = mbar_wait_in<kInt4>(bar_ofree, (pv_items - 1) & 1, p.wait_ns);   // the softmax warps have read the previous item's O
             ok = __all_sync(kFullMask, ok);     // keep the warp converged on a timeout
             if (!ok) break;                     // gave up: nothing more is issued
             tc_fence_after();
             {
-                uint32_t v_w = v_lo0 + s * kSlotStep;
+                uint32_t v_w = v_lo0 + vslot * kSlotStep;
                 uint32_t p_col = tmem_base + s * kTcTile;
                 const uint32_t o_col = tmem_base + tmem_o_col;
                 uint32_t acc_o = pv_j > 0 ? 1u : 0u;
@@ -442,7 +750,7 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
                 }
             }
             if (elect_one()) tc_commit(bar_o + 8 * s);
-            if (elect_one()) tc_commit(bar_empty_v + 8 * s);
+            if (elect_one()) tc_commit(bar_empty_v + 8 * vslot);
             if (++pv_j == pv_n) { ++pv_item; ++pv_items; pv_j = 0; pv_n = tiles_of(pv_item); }
             issue_qk_upto(g);
             if (++s == R) { s = 0; ph ^= 1; }
@@ -453,9 +761,11 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
             // that (bounded) before the CTA frees its tensor memory.
             if (lane == 0 && p.status) atomicExch(p.status, 13);
             if (elect_one()) tc_commit(bar_drain);
-            mbar_wait(bar_drain, 0, p.wait_ns);
+            mbar_wait_in<kInt4>(bar_drain, 0, p.wait_ns);
         }
+    }
     } else {
+    if constexpr (kInt4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcSoftmaxRegs));
     // ---- softmax warps ---------------------------------------------------------------------------
     // Thread (half, quad, lane) owns row r = 32 quad + lane (TMEM lane r) and the token columns
     // [32 half, 32 half + 32) of every tile; the two threads of a row exchange their maxima through
@@ -465,7 +775,8 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
     const int r = quad * 32 + lane;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t tmem_o = lane_addr + tmem_o_col + half * OC;
-    const float c = p.scale_log2;
+    // from products to powers of two (kInt4: the scores carry the factor already)
+    const float c = kInt4 ? 1.f : p.scale_log2;
     bool ok = true;
     int t = 0;                                  // running tile index (all rings)
     int s = 0;                                  // t % R and the phase bit (t / R) & 1, kept incrementally
@@ -474,7 +785,7 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
     uint32_t o_ph = 0;
     auto ensure_o = [&](int upto) {             // every o_done phase is consumed exactly once, in order
         while (o_seen < upto) {
-            if (ok) ok = mbar_wait(bar_o + 8 * o_slot, o_ph, p.wait_ns);
+            if (ok) ok = mbar_wait_in<kInt4>(bar_o + 8 * o_slot, o_ph, p.wait_ns);
             ++o_seen;
             if (++o_slot == R) { o_slot = 0; o_ph ^= 1; }
         }
@@ -537,9 +848,32 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
             mbar_arrive(bar_q);
         }
 
+        float q_sum = 0.f;
+        if constexpr (kInt4) {
+            // Sum of the row's elements: each thread adds up the half it wrote (its own asynchronous copies have
+            // landed after the wait) while the item's first product is on its way; the partner has the rest.
+            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const int ch = half * (D / 16) + i;
+                const uint4 v = *reinterpret_cast<const uint4*>(tc_smem + L::kQOff + (ch >> 3) * (128 * 128) + swz128(r, ch & 7));
+                const float2 e0 = Int4Elt<T>::unpack(v.x), e1 = Int4Elt<T>::unpack(v.y), e2 = Int4Elt<T>::unpack(v.z), e3 = Int4Elt<T>::unpack(v.w);
+                q_sum += ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+            }
+            // same buffer discipline as the maxima below: this parity was last read before the partner's last barrier
+            float* xbuf = xch + ((t + 1) & 1) * 256;
+            xbuf[half * 128 + r] = q_sum;
+            pair_sync();
+            q_sum += xbuf[(half ^ 1) * 128 + r];
+            pair_sync();
+        }
+
         float m_used = -INFINITY, l = 0.f;
         for (int j = 0; j < n_tiles; ++j, ++t) {
-            if (ok) ok = mbar_wait(bar_s + 8 * s, ph, p.wait_ns);
+            if (ok) ok = mbar_wait_in<kInt4>(bar_s + 8 * s, ph, p.wait_ns);
+            if constexpr (kInt4) {
+                if (ok) ok = mbar_wait_in<kInt4>(bar_prm + 8 * (t & 3), (t >> 2) & 1, p.wait_ns);     // long done: before the K tile was full
+            }
             tc_fence_after();
             if (j == n_tiles - 1 && item + 1 < item_hi) {
                 // Last tile of the item.  Its S has completed, and with it every Q K^T of the item:
@@ -567,6 +901,19 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
             constexpr int CH = kTcTile / 2;     // token columns per thread
             float sc[CH];
             tmem_ld_f<CH>(lane_addr + s * kTcTile + half * CH, sc);
+            if constexpr (kInt4) {
+                const float* prm = reinterpret_cast<const float*>(tc_smem + L::kPrmOff) + (t & 3) * 256 + half * CH;
+                const uint64_t qq = pack_f32x2(q_sum, q_sum);
+#pragma unroll
+                for (int i = 0; i < CH; i += 4) {       // (the same address in every lane: broadcasts)
+                    const float4 f = *reinterpret_cast<const float4*>(prm + i);
+                    const float4 a = *reinterpret_cast<const float4*>(prm + 128 + i);
+                    const uint64_t lo = fma_f32x2(pack_f32x2(sc[i], sc[i + 1]), pack_f32x2(f.x, f.y), mul_f32x2(pack_f32x2(a.x, a.y), qq));
+                    const uint64_t hi = fma_f32x2(pack_f32x2(sc[i + 2], sc[i + 3]), pack_f32x2(f.z, f.w), mul_f32x2(pack_f32x2(a.z, a.w), qq));
+                    unpack_f32x2(lo, sc[i], sc[i + 1]);
+                    unpack_f32x2(hi, sc[i + 2], sc[i + 3]);
+                }
+            }
             const int valid = min(kTcTile, kv_len - j * kTcTile);
             const int row_valid = kLimits ? min(valid, row_limit - j * kTcTile) : valid;
             if (row_valid < kTcTile) {
@@ -616,10 +963,10 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
             l += sum0 + sum1;
             // P over the S columns this row has consumed: CH / 2 packed columns per half
             tmem_st32(lane_addr + s * kTcTile + half * (CH / 2), packed);
-            if (valid < kTcTile) {
+            if (!kInt4 && valid < kTcTile) {
                 // V rows past the valid tokens may hold anything (stale tiles, never written pages):
                 // zero them (once the tile's V has landed) so that P = 0 times garbage cannot make a NaN
-                if (ok) ok = mbar_wait(bar_full_v + 8 * s, ph, p.wait_ns);
+                if (ok) ok = mbar_wait_in<kInt4>(bar_full_v + 8 * s, ph, p.wait_ns);
                 const int rows = kTcTile - valid;
                 const int chunks = rows * 8 * L::kBoxes;
                 for (int i = tid; i < chunks; i += kSW * 32) {
@@ -656,7 +1003,9 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
                 const int qi = r / p.hratio, gg = r - qi * p.hratio;
                 slot = static_cast<size_t>(entry_base + qi) * p.hratio + gg;
             }
-            const float inv = (!kLimits || l_row > 0.f) ? 1.f / l_row : 0.f;    // a row that saw nothing
+            // a row that saw nothing has l = 0 (kInt4: a NaN it has seen must not pass for that)
+            const bool seen = !kLimits || (kInt4 ? l_row != 0.f : l_row > 0.f);
+            const float inv = seen ? 1.f / l_row : 0.f;
             float ov[OC];
             tmem_ld_f<OC>(tmem_o, ov);
             tc_fence_before();
@@ -673,7 +1022,7 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
                                    "f"(ov[8 * i + 6] * inv), "f"(ov[8 * i + 7] * inv)
                                  : "memory");
                 if (half == 0)
-                    p.part_lse[slot] = (!kLimits || l_row > 0.f) ? m_used * p.scale + logf(l_row) : -INFINITY;
+                    p.part_lse[slot] = seen ? m_used * (kInt4 ? 0.6931471805599453f : p.scale) + logf(l_row) : -INFINITY;
             }
         }
         rec_a = next_a;
@@ -688,6 +1037,18 @@ dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap
     __syncthreads();
     if (warp == 0) tmem_dealloc(tmem_base, kTcTmemCols);
     if (tid == 0) count_out();
+}
+
+template <typename T, int D, bool kLimits>
+__global__ void __launch_bounds__(kTcThreads, 1)
+dense_tc_kernel(const DenseTcParams dp, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    dense_tc_body<T, D, kLimits, false>(dp, &kmap, &vmap, Int4Cache{});
+}
+
+// The same over a 4-bit cache.
+template <typename T, int D, bool kLimits>
+__global__ void __launch_bounds__(kTcInt4Threads, 1) dense_tc_int4_kernel(const DenseTcParams dp, const Int4Cache cache) {
+    dense_tc_body<T, D, kLimits, true>(dp, nullptr, nullptr, cache);
 }
 
 }  // namespace pat

@@ -54,7 +54,7 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 constexpr uint64_t kDefaultWaitNs = 1000ull * 1000ull * 1000ull;
 // The polling loop is kept out of line: a kernel waits in many places, and warps that run a
 // little code per tile (TMA producers, the MMA issuer) are bound by instruction fetch.
-static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
     const uint64_t start = global_timer_ns();
     for (uint32_t i = 1; i < kMaxPolls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -62,9 +62,18 @@ static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity
     }
     return false;
 }
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+    return mbar_poll(bar, parity, limit_ns);
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
     if (mbar_try_wait(bar, parity)) return true;
     return mbar_wait_slow(bar, parity, limit_ns);
+}
+// In a kernel whose warpgroups have different register counts (setmaxnreg) no function may be called, and
+// the loop stays in line.
+template <bool kInline> __device__ __forceinline__ bool mbar_wait_in(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+    if constexpr (kInline) return mbar_try_wait(bar, parity) || mbar_poll(bar, parity, limit_ns);
+    else return mbar_wait(bar, parity, limit_ns);
 }
 // After a wait has given up: a short second chance (about 20 us) for copies or products that
 // are still on their way, so that nothing lands in memory the CTA has already handed back.

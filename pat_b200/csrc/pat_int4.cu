@@ -11,6 +11,7 @@
 #include <cfloat>
 #include <cmath>
 
+#include "pat_dense_tc.cuh"
 #include "pat_int4.cuh"
 
 namespace {
@@ -332,7 +333,32 @@ template <typename T, int D> int launch_attention(const pat_decode_int4_args& a,
     p.wait_ns = a.wait_limit_us > 0 ? static_cast<uint64_t>(a.wait_limit_us) * 1000ull : kDefaultWaitNs;
     const Int4Cache cache{static_cast<const unsigned char*>(a.kv_cache), a.page_stride, a.head_stride};
 
-    if (a.work.num_stream_items > 0) {
+    // The order of the 16-bit path: dense kernel, streaming kernel as its programmatic dependent, merge (which
+    // waits for the last dense CTA through a control word of the workspace).
+    const bool streaming = a.work.num_stream_items > 0 && !(a.flags & PAT_SKIP_STREAM);
+    const bool dense = a.work.num_dense_items > 0 && !(a.flags & PAT_SKIP_DENSE);
+    const bool merge = !(a.flags & PAT_SKIP_MERGE);
+    const bool overlap = streaming && dense && !(a.flags & PAT_NO_OVERLAP);
+    int32_t* sync = overlap && merge ? static_cast<int32_t*>(a.workspace) : nullptr;
+    if (dense) {
+        static std::atomic<bool> configured[kMaxDevices][2];
+        auto kern = limits ? dense_tc_int4_kernel<T, D, true> : dense_tc_int4_kernel<T, D, false>;
+        constexpr int smem = TcSmem<D, true>::kRequest;
+        if (!configured[dev][limits].load(std::memory_order_acquire)) {
+            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return PAT_ERR_CUDA;
+            configured[dev][limits].store(true, std::memory_order_release);
+        }
+        DenseTcParams dp{};
+        dp.a = p;
+        dp.a.items = p.items + static_cast<size_t>(a.work.num_stream_items) * 8;
+        dp.a.num_items = a.work.num_dense_items;
+        dp.cta_begin = a.work_blob + a.work.dense_cta_off;
+        dp.dense_q = a.work_blob + a.work.dense_q_off;
+        dp.dense_q_width = a.work.dense_q_width;
+        dp.sync = sync;
+        kern<<<static_cast<unsigned>(a.work.num_dense_ctas), kTcInt4Threads, smem, stream>>>(dp, cache);
+    }
+    if (streaming) {
         static std::atomic<bool> configured[kMaxDevices][2];
         auto kern = limits ? int4_stream_kernel<T, D, true> : int4_stream_kernel<T, D, false>;
         constexpr int smem = int4_stream_smem_bytes<D>();
@@ -340,11 +366,23 @@ template <typename T, int D> int launch_attention(const pat_decode_int4_args& a,
             if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return PAT_ERR_CUDA;
             configured[dev][limits].store(true, std::memory_order_release);
         }
-        const long long grid = static_cast<long long>(p.num_items) * a.num_kv_heads;
+        const long long grid = (static_cast<long long>(p.num_items) * a.num_kv_heads + kInt4Warps - 1) / kInt4Warps;
         if (grid > 0x7fffffffLL) return PAT_ERR_TOO_LARGE;
-        kern<<<static_cast<unsigned>(grid), kInt4Warps * 32, smem, stream>>>(p, cache);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(grid));
+        cfg.blockDim = dim3(kInt4Warps * 32);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = overlap ? 1 : 0;
+        if (cudaLaunchKernelEx(&cfg, kern, p, cache) != cudaSuccess) return PAT_ERR_CUDA;
     }
+    if (!merge) return cudaGetLastError() == cudaSuccess ? PAT_OK : PAT_ERR_CUDA;
     MergeParams mp{};
+    mp.sync = sync;
     mp.status = a.status_word;
     mp.wait_ns = p.wait_ns;
     mp.part_o = part_o;
@@ -413,7 +451,7 @@ int pat_b200_decode_int4(const pat_decode_int4_args* args, void* stream_handle) 
         return PAT_ERR_BAD_PLAN;
     if (a.work.hratio != a.num_q_heads / a.num_kv_heads || a.work.page_size != a.page_size || a.work.kv_heads != a.num_kv_heads)
         return PAT_ERR_BAD_PLAN;
-    if (a.work.max_page_id >= a.num_pages || a.work.num_dense_items > 0) return PAT_ERR_BAD_PLAN;
+    if (a.work.max_page_id >= a.num_pages) return PAT_ERR_BAD_PLAN;
     if (a.head_dim != 64 && a.head_dim != 128) return PAT_ERR_UNSUPPORTED;
     if (a.dtype != PAT_DTYPE_FP16 && a.dtype != PAT_DTYPE_BF16) return PAT_ERR_UNSUPPORTED;
     if (a.page_size < 16 || a.page_size % 16 != 0 || a.page_size > 256) return PAT_ERR_UNSUPPORTED;

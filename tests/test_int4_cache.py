@@ -315,20 +315,23 @@ def _batch(kind, page, seed):
 
 
 def _bounds(k, v, q, scale, dtype, ref):
-    """Largest errors of output and LSE.  With u = half a step of the type: P' = p s is rounded once
-    (relative u), which moves sum p s c by at most u times the largest s c = v - lo; the output is rounded
-    once (u |out|).  A score is an fp32 sum of 2 D products of at most |q| (16 + 15) s: 2 D roundings
-    of 2^-24 of their sum bound it, and a score's error e changes a weight by a factor of 1 + 2 e, the
-    output by at most 2 e times the spread of the values.  exp2 and the sums over tokens and
-    parts are fp32 as well: 2^-20 of the spread covers them for the lengths used here (below 2^10 terms in a
-    random walk, 2^-24 each)."""
+    """Largest errors of output and LSE.  With u = half a step of the type:
+
+    * Few rows: P' = p s is rounded once (relative u) and multiplies c - 7.5, which moves sum p s (c - 7.5) by
+      at most u times half the spread of a value row.  Many rows: p and v = lo + s c are rounded once each, which
+      moves sum p v by at most 2 u max |v|.  The output is rounded once (u |out|).
+    * A score is an fp32 sum of 2 D products of at most |q| (16 + 15) s (the codes are exact on both paths):
+      2 D roundings of 2^-24 of their sum bound it, and a score's error e changes a weight by a factor of
+      1 + 2 e, the output by at most 2 e times the spread of the values.
+    * exp2 and the sums over tokens and parts are fp32 as well: 2^-20 of the spread covers them for the lengths used
+      here (below 2^10 terms in a random walk, 2^-24 each)."""
     D = q.shape[-1]
     u = torch.finfo(dtype).eps / 2
     spread_v = float((v.amax(-1) - v.amin(-1)).max())
     top_v = float(v.abs().max())
     span_k = float(((v.abs().amax(-1) * 0 + (k.amax(-1) - k.amin(-1)) / 15 * 31) + k.abs().amax(-1)).max())
     e = 2 * D * 2.0 ** -24 * float(q.double().abs().sum(-1).max()) * span_k * scale
-    return u * (spread_v + ref.abs()) + (2 * e + 2.0 ** -20) * 2 * top_v, e + 2.0 ** -20 * 16
+    return u * (max(spread_v / 2, 2 * top_v) + ref.abs()) + (2 * e + 2.0 ** -20) * 2 * top_v, e + 2.0 ** -20 * 16
 
 
 def _check(dtype, hq, hk, d, page, lens, tables, pages, T=1, seed=0, scale=None, cache=None, spread=0.5, q=None):
