@@ -76,12 +76,21 @@ def set_default_config(cfg: Optional[WorkConfig]) -> None:
 
 
 def int4_config() -> WorkConfig:
-    """Options of the work lists for a 4-bit cache."""
+    """Options of the work lists for a 4-bit cache.
+
+    A warp of the streaming kernel takes 8 rows, and a unit is a warp's, not a CTA's: smaller chunks, more of
+    them (128 tokens and 16 per SM against the 16-bit path's 256 and 4: small batch 12.6 -> 8.4 us, deep tree even,
+    long contexts even).  Unpacking a tile costs the dense kernel the same for one row as for 128, so it gets
+    segments of 33 rows on (17: small batch 29 us against 13, two-level tree 69 against 61, deep tree 99
+    against 93; 49 and 65 are even), cut for every SM: neither kernel waits for memory long enough to gain
+    from running beside the other (long contexts 740 us on the 16-bit path's share of the SMs, 535 on all of
+    them).  Figures in microseconds per step on a B200."""
     cfg = WorkConfig(**{n: getattr(default_config(), n) for n in WorkConfig.__slots__})
     cfg.stream_rows = cfg.stream_rows or 8
     cfg.items_per_sm = cfg.items_per_sm or 16
     cfg.chunk_tokens_min = cfg.chunk_tokens_min or 128
     cfg.dense_tile_ns = cfg.dense_tile_ns or -1
+    cfg.dense_min_rows = cfg.dense_min_rows or 33
     return cfg
 
 

@@ -12,7 +12,7 @@
 // every warp sorts its 32 - collect the few that reach it, and order those by counting.
 //
 // Candidates of different beams are compared by a value that contains two log-sums, so these are
-// kept to about 1e-8: exponentials in fp32 with the argument in two parts, sums of at most 32 of them
+// kept to about 1e-8: exponentials in fp32 with log2(e) in two parts, sums of at most 32 of them
 // in fp32, everything above in fp64.  Which thread adds which logit depends on the index alone, not on
 // where a row starts in memory: equal rows give equal sums, and equal candidates meet as ties.
 #include <cuda_bf16.h>
@@ -44,11 +44,11 @@ struct BeamParams {
     float* out_scores;             // [batch, num_out]
     int32_t* out_parents;
     int32_t* out_tokens;
-    // scratch, per (row, chunk): the chunk's largest logits in order, their number, its maximum and sum
+    // scratch, per (row, chunk): the chunk's largest logits in order, their number, its sum
     float* list_x;                 // [rows][chunks][num_out]
     int32_t* list_v;
     int32_t* list_n;               // [rows][chunks]
-    float* chunk_max;
+    float* chunk_ref;              // reference of the sum, in powers of two; +inf: NaN or +inf seen, -inf: nothing but -inf
     double* chunk_sum;
     int batch, beams, vocab, num_out, chunks, chunk_len, pad_token;
 };
@@ -58,12 +58,18 @@ template <> __device__ __forceinline__ float to_float<float>(float v) { return v
 template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// exp(d) for d <= 0, argument d * log2(e) in two parts
-__device__ __forceinline__ float exp_neg(float d) {
-    constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500011e-08f;
+// 2^(x log2(e) - ref), log2(e) in two parts.  The reference is whatever float lies near the largest x log2(e), and the
+// sums are exact about it: nothing but the rounding of each argument is lost.
+constexpr float kLog2eHi = 1.44269502162933349609375f, kLog2eLo = 1.925963033500011e-08f;
+__device__ __forceinline__ float exp2_about(float x, float ref) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, kHi, d * kLo)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(x, kLog2eHi, fmaf(x, kLog2eLo, -ref))));
     return y;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 // a is preferred to b: larger value, or equal and lower index
@@ -107,7 +113,7 @@ __device__ __forceinline__ float warp_sorted(float v, int lane) {
     return v;
 }
 
-template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 3) beam_scan_kernel(const BeamParams p) {
+template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 5) beam_scan_kernel(const BeamParams p) {
     constexpr int kPer = kGroups * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int64_t row = blockIdx.x / p.chunks;
@@ -119,7 +125,7 @@ template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 3
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     __shared__ float s_max[kWarps], s_edge[kWarps];
     __shared__ double s_sum[kWarps];
-    __shared__ int s_bad[kWarps], s_count;
+    __shared__ int s_count;
     __shared__ float s_x[kListCap];
     __shared__ int s_v[kListCap];
     if (tid == 0) s_count = 0;
@@ -141,32 +147,46 @@ template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 3
         }
     }
     auto token_of = [&](int i) { return base + (i >> 3) * (kThreads * 8) + tid * 8 + (i & 7); };
-    float top = -INFINITY;
-    bool bad = false;
+    float group[kGroups], top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        top = fmaxf(top, x[i]);
-        bad = bad || !(x[i] < INFINITY);           // NaN or +inf: the beam takes no part
+    for (int gi = 0; gi < kGroups; ++gi) {
+        group[gi] = x[gi * 8];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) group[gi] = max_or_nan(group[gi], x[gi * 8 + i]);
+        top = max_or_nan(top, group[gi]);
     }
     // At least q of every warp's maxima reach `edge`, so at least num_out logits of the chunk do.
     const int q = (p.num_out + kWarps - 1) / kWarps;
+    const bool bad = __any_sync(kFull, !(top < INFINITY));      // NaN or +inf: the beam takes no part
     const float sorted = warp_sorted(top, lane);
-    const bool any_bad = __any_sync(kFull, bad);
-    if (lane == 0) { s_max[warp] = sorted; s_bad[warp] = any_bad; }
+    if (lane == 0) s_max[warp] = bad ? INFINITY : sorted;
     if (lane == q - 1) s_edge[warp] = sorted;
     __syncthreads();
     float m = s_max[0], edge = s_edge[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) { m = fmaxf(m, s_max[w]); edge = fminf(edge, s_edge[w]); }
+    const size_t slot = static_cast<size_t>(row) * p.chunks + chunk;
+    if (!(m < INFINITY) || m == -INFINITY) {       // uniform: nothing to sum, nothing to list
+        if (tid == 0) {
+            p.chunk_ref[slot] = m;                 // +inf: bad, -inf: empty
+            p.list_n[slot] = 0;
+        }
+        return;
+    }
 
+    const float ref = m * kLog2eHi;
     float sum = 0.f;
-    if (m > -INFINITY) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            sum += exp_neg(x[i] - m);
-            if (x[i] >= edge && x[i] > -INFINITY) {
-                const int at = atomicAdd(&s_count, 1);
-                if (at < kListCap) { s_x[at] = x[i]; s_v[at] = token_of(i); }
+    for (int gi = 0; gi < kGroups; ++gi) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += exp2_about(x[gi * 8 + i], ref);
+        if (group[gi] >= edge && group[gi] > -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (x[gi * 8 + i] >= edge && x[gi * 8 + i] > -INFINITY) {
+                    const int at = atomicAdd(&s_count, 1);
+                    if (at < kListCap) { s_x[at] = x[gi * 8 + i]; s_v[at] = token_of(gi * 8 + i); }
+                }
             }
         }
     }
@@ -176,24 +196,26 @@ template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 3
     if (lane == 0) s_sum[warp] = total;
     __syncthreads();
     const int found = s_count;
-    const size_t slot = static_cast<size_t>(row) * p.chunks + chunk;
     float* out_x = p.list_x + slot * p.num_out;
     int32_t* out_v = p.list_v + slot * p.num_out;
     if (tid == 0) {
         double z = 0.0;
-        int any = 0;
-        for (int w = 0; w < kWarps; ++w) { z += s_sum[w]; any |= s_bad[w]; }
-        p.chunk_max[slot] = any ? NAN : m;
+        for (int w = 0; w < kWarps; ++w) z += s_sum[w];
+        p.chunk_ref[slot] = ref;
         p.chunk_sum[slot] = z;
         p.list_n[slot] = found < p.num_out ? found : p.num_out;
     }
     if (found <= kListCap) {
-        for (int i = tid; i < found; i += kThreads) {
-            const float xi = s_x[i];
-            const int vi = s_v[i];
+        // place of a candidate = how many are preferred to it; four threads count for each
+        for (int i0 = 0; i0 < found; i0 += kThreads / 4) {
+            const int i = i0 + tid / 4;
+            const float xi = i < found ? s_x[i] : 0.f;
+            const int vi = i < found ? s_v[i] : 0;
             int r = 0;
-            for (int j = 0; j < found; ++j) r += before(s_x[j], s_v[j], xi, vi) ? 1 : 0;
-            if (r < p.num_out) { out_x[r] = xi; out_v[r] = vi; }
+            for (int j = tid & 3; j < found; j += 4) r += before(s_x[j], s_v[j], xi, vi) ? 1 : 0;
+            r += __shfl_xor_sync(kFull, r, 1);
+            r += __shfl_xor_sync(kFull, r, 2);
+            if ((tid & 3) == 0 && i < found && r < p.num_out) { out_x[r] = xi; out_v[r] = vi; }
         }
         return;
     }
@@ -241,74 +263,81 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p)
     s_used[tid] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
+    // log-sum of every beam: ln 2 * (ref + log2 sum)
     for (int k = warp; k < p.beams; k += kWarps) {
         double shift = NAN;
         if (beam_is_live(p, b, k)) {
             const size_t slot = (static_cast<size_t>(b) * p.beams + k) * p.chunks;
             float m = -INFINITY;
-            bool bad = false;
-            for (int c = lane; c < p.chunks; c += 32) {
-                const float cm = p.chunk_max[slot + c];
-                bad = bad || cm != cm;
-                m = fmaxf(m, cm);
-            }
+            for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.chunk_ref[slot + c]);
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
-            bad = __any_sync(kFull, bad);
-            if (!bad && m > -INFINITY) {
+            if (m < INFINITY && m > -INFINITY) {
                 double z = 0.0;
                 for (int c = lane; c < p.chunks; c += 32) {
-                    const float cm = p.chunk_max[slot + c];
-                    if (cm > -INFINITY) z += p.chunk_sum[slot + c] * exp(static_cast<double>(cm) - static_cast<double>(m));
+                    const float ref = p.chunk_ref[slot + c];
+                    if (ref > -INFINITY) z += p.chunk_sum[slot + c] * exp2(static_cast<double>(ref) - static_cast<double>(m));
                 }
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) z += __shfl_xor_sync(kFull, z, d);
-                shift = static_cast<double>(p.scores[b * p.score_stride + k]) - (static_cast<double>(m) + log(z));
+                shift = static_cast<double>(p.scores[b * p.score_stride + k]) - 0.693147180559945309417 * (static_cast<double>(m) + log2(z));
             }
         }
         if (lane == 0) s_shift[k] = shift;
     }
     __syncthreads();
 
-    // Candidates: the lists' places one after the other, then one per beam for those that are finished.
-    const int64_t listed = static_cast<int64_t>(p.beams) * p.chunks * p.num_out;
-    const int64_t total = listed + p.beams;
-    auto candidate = [&](int64_t j, double& val, int64_t& idx) -> bool {
-        if (j < listed) {
-            const int64_t list = j / p.num_out;
-            const int pos = static_cast<int>(j - list * p.num_out), k = static_cast<int>(list / p.chunks);
-            const double shift = s_shift[k];
-            const size_t slot = static_cast<size_t>(b) * p.beams * p.chunks + list;
-            if (shift != shift || pos >= p.list_n[slot]) return false;
-            val = shift + static_cast<double>(p.list_x[slot * p.num_out + pos]);
-            idx = static_cast<int64_t>(k) * p.vocab + p.list_v[slot * p.num_out + pos];
-            return true;
+    // Candidates: the places of all lists, then one candidate per finished beam.
+    const int lists = p.beams * p.chunks;
+    const int shift_out = 32 - __clz(p.num_out - 1 | 1);       // places per list, rounded up to a power of two
+    const int total = (lists << shift_out) + (p.finished ? p.beams : 0);
+    const float* my_x = p.list_x + static_cast<size_t>(b) * lists * p.num_out;
+    const int32_t* my_v = p.list_v + static_cast<size_t>(b) * lists * p.num_out;
+    auto value_of = [&](int j) -> double {                     // -inf: no candidate
+        const int list = j >> shift_out, pos = j & ((1 << shift_out) - 1);
+        if (list < lists) {
+            if (pos >= p.num_out) return -INFINITY;
+            const float x = my_x[list * p.num_out + pos];      // (may hold anything behind the list's end)
+            const int n = p.list_n[static_cast<size_t>(b) * lists + list];
+            const double shift = s_shift[list / p.chunks];
+            return pos < n && shift == shift ? shift + static_cast<double>(x) : -INFINITY;
         }
-        const int k = static_cast<int>(j - listed);
-        if (!p.finished || !p.finished[b * p.finished_stride + k]) return false;
-        const float sc = p.scores[b * p.score_stride + k];
-        if (!isfinite(sc)) return false;
-        val = sc;
-        idx = static_cast<int64_t>(k) * p.vocab + p.pad_token;
-        return true;
+        const int k = j - (lists << shift_out);
+        const float score = p.scores[b * p.score_stride + k];
+        return p.finished[b * p.finished_stride + k] && isfinite(score) ? static_cast<double>(score) : -INFINITY;
     };
-    double val;
-    int64_t idx;
+    auto index_of = [&](int j) -> int64_t {
+        const int list = j >> shift_out, pos = j & ((1 << shift_out) - 1);
+        if (list < lists) return static_cast<int64_t>(list / p.chunks) * p.vocab + my_v[list * p.num_out + pos];
+        return static_cast<int64_t>(j - (lists << shift_out)) * p.vocab + p.pad_token;
+    };
+    // the first kKeep values of every thread stay in registers between the two passes
+    constexpr int kKeep = 8;
+    double kept[kKeep];
     float top = -INFINITY;
-    for (int64_t j = tid; j < total; j += kThreads)
-        if (candidate(j, val, idx)) top = fmaxf(top, __double2float_rd(val));
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+        const int j = tid + i * kThreads;
+        kept[i] = j < total ? value_of(j) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) top = fmaxf(top, __double2float_rd(kept[i]));
+    for (int j = tid + kKeep * kThreads; j < total; j += kThreads) top = fmaxf(top, __double2float_rd(value_of(j)));
     const float sorted = warp_sorted(top, lane);
     if (lane == (p.num_out + kWarps - 1) / kWarps - 1) s_edge[warp] = sorted;
     __syncthreads();
     float edge = s_edge[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) edge = fminf(edge, s_edge[w]);
-    for (int64_t j = tid; j < total; j += kThreads) {
-        if (candidate(j, val, idx) && val >= static_cast<double>(edge)) {
+    auto collect = [&](int j, double val) {
+        if (val > -INFINITY && val >= static_cast<double>(edge)) {
             const int at = atomicAdd(&s_count, 1);
-            if (at < kListCap) { s_val[at] = val; s_idx[at] = idx; }
+            if (at < kListCap) { s_val[at] = val; s_idx[at] = index_of(j); }
         }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) collect(tid + i * kThreads, kept[i]);
+    for (int j = tid + kKeep * kThreads; j < total; j += kThreads) collect(j, value_of(j));
     __syncthreads();
     const int found = s_count;
     auto put = [&](int n, double v, int64_t i) {
@@ -317,13 +346,18 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p)
         p.out_tokens[b * p.num_out + n] = static_cast<int32_t>(i % p.vocab);
     };
     if (found <= kListCap) {
-        for (int i = tid; i < found; i += kThreads) {
-            const double vi = s_val[i];
-            const int64_t ii = s_idx[i];
+        for (int i0 = 0; i0 < found; i0 += kThreads / 4) {
+            const int i = i0 + tid / 4;
+            const double vi = i < found ? s_val[i] : 0.0;
+            const int64_t ii = i < found ? s_idx[i] : 0;
             int r = 0;
-            for (int j = 0; j < found; ++j) r += before(s_val[j], s_idx[j], vi, ii) ? 1 : 0;
-            if (r < p.num_out) put(r, vi, ii);
-            if (ii < 2 * kMaxOut) s_used[ii] = 1;
+            for (int j = tid & 3; j < found; j += 4) r += before(s_val[j], s_idx[j], vi, ii) ? 1 : 0;
+            r += __shfl_xor_sync(kFull, r, 1);
+            r += __shfl_xor_sync(kFull, r, 2);
+            if ((tid & 3) == 0 && i < found) {
+                if (r < p.num_out) put(r, vi, ii);
+                if (ii < 2 * kMaxOut) s_used[ii] = 1;
+            }
         }
         if (found >= p.num_out) return;
         // Fewer finite values than asked for, and all of them are listed: the rest are -inf, all equal, so the
@@ -340,8 +374,12 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p)
     for (int n = 0; n < p.num_out; ++n) {
         double best = -INFINITY;
         int64_t best_idx = INT64_MAX;
-        for (int64_t j = tid; j < total; j += kThreads)
-            if (candidate(j, val, idx) && before(last, last_idx, val, idx) && before(val, idx, best, best_idx)) { best = val; best_idx = idx; }
+        for (int j = tid; j < total; j += kThreads) {
+            const double val = value_of(j);
+            if (val == -INFINITY || !(val < last || (val == last && index_of(j) > last_idx))) continue;
+            const int64_t idx = index_of(j);
+            if (before(val, idx, best, best_idx)) { best = val; best_idx = idx; }
+        }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) {
             const double ov = __shfl_xor_sync(kFull, best, d);
@@ -380,7 +418,8 @@ int beam_shape(int batch, int beams, int vocab, int num_out) {
     if (num_out > static_cast<int64_t>(beams) * vocab) return PAT_ERR_BAD_ARGUMENT;
     if (num_out > kMaxOut || beams > kMaxBeams || vocab > (1 << 24)) return PAT_ERR_TOO_LARGE;
     const int64_t rows = static_cast<int64_t>(batch) * beams;
-    if (rows * cut_rows(rows, vocab).chunks > 0x7fffffffLL) return PAT_ERR_TOO_LARGE;
+    const int64_t chunks = cut_rows(rows, vocab).chunks;
+    if (rows * chunks > 0x7fffffffLL || beams * chunks * kMaxOut > 0x3fffffffLL) return PAT_ERR_TOO_LARGE;
     return PAT_OK;
 }
 
@@ -441,7 +480,7 @@ extern "C" int pat_b200_beam_select(const pat_beam_args* args, void* stream_hand
     ws += align256(lists * a.num_out * 4);
     p.list_n = reinterpret_cast<int32_t*>(ws);
     ws += align256(lists * 4);
-    p.chunk_max = reinterpret_cast<float*>(ws);
+    p.chunk_ref = reinterpret_cast<float*>(ws);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
     const unsigned grid = static_cast<unsigned>(lists);
     void (*scan)(BeamParams);

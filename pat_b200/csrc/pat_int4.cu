@@ -29,6 +29,7 @@ struct RowsParams {            // append and read-back: rows of 16-bit elements 
     int64_t page_stride, head_stride;                         // bytes
     int64_t num_slots;                                        // pages * page_size
     int num_tokens, heads, page_size;
+    int heads_per_cta;
 };
 
 // Byte offsets, from the start of a tile, of the codes of dims 8i .. 8i + 7 of token `tok`: one word of K,
@@ -40,19 +41,19 @@ template <int D> __device__ __forceinline__ int v_half_off(int tok, int i) {
     return Int4Tile<D>::kVOff + (tok >> 3) * 4 * D + (g * 4 + ((tok & 7) >> 1)) * Int4Tile<D>::kLaneBytes + wh * 8 + (tok & 1) * 2;
 }
 
-// Both kernels: one CTA = 16 consecutive tokens of the call x one KV head (heads next to each other: they
-// share the tokens' rows).  When the 16 slots are one tile in order - a prefill chunk, a cached prefix - the
-// tile passes through shared memory and is moved by 16-byte accesses; otherwise every row goes to its place by
+// Both kernels: one CTA = 16 consecutive tokens of the call x some KV heads, one after the other, the next head's bytes
+// on their way while one is worked on.  When the 16 slots are one tile in order - a prefill chunk, a cached prefix -
+// the tile passes through shared memory and is moved by 16-byte accesses; otherwise every row goes to its place by
 // itself, V in 2-byte pieces (a token owns 16-bit halves of the V words).
 constexpr int kRowThreads = 256;
 
 struct TileGroup {
     int64_t slot[16];          // -1: padding, or outside the cache
-    unsigned char* tile;       // the one tile of a whole run, or null
+    unsigned char* tile;       // head 0's tile of a whole run, or null
 };
 
 // All threads call this; `grp` is shared memory.
-template <int D> __device__ __forceinline__ void load_group(const RowsParams& p, TileGroup& grp, int token0, int head) {
+template <int D> __device__ __forceinline__ void load_group(const RowsParams& p, TileGroup& grp, int token0) {
     if (threadIdx.x < 32) {
         const int t = threadIdx.x;
         int64_t slot = -1;
@@ -67,8 +68,7 @@ template <int D> __device__ __forceinline__ void load_group(const RowsParams& p,
             unsigned char* tile = nullptr;
             if (run) {
                 const int64_t page = first / p.page_size;
-                tile = p.cache + page * p.page_stride + head * p.head_stride +
-                       ((first - page * p.page_size) >> 4) * Int4Tile<D>::kBytes;
+                tile = p.cache + page * p.page_stride + ((first - page * p.page_size) >> 4) * Int4Tile<D>::kBytes;
             }
             grp.tile = tile;
         }
@@ -87,34 +87,78 @@ template <typename T> __device__ __forceinline__ float elt_round(float x);
 template <> __device__ __forceinline__ float elt_round<__nv_bfloat16>(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 template <> __device__ __forceinline__ float elt_round<__half>(float x) { return __half2float(__float2half_rn(x)); }
 
-// The codes of 8 elements: low half dims 0, 2, 4, 6, high half 1, 3, 5, 7.
+// Smallest and largest of two pairs, NaN if one holds a NaN.
+template <typename T> __device__ __forceinline__ void min_max_pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    using V = typename Pack2<T>::V;
+    const V v = *reinterpret_cast<const V*>(&w), l = __hmin2_nan(v, *reinterpret_cast<const V*>(&lo)),
+            h = __hmax2_nan(v, *reinterpret_cast<const V*>(&hi));
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The codes of 16 elements: per 8 of them, low half dims 0, 2, 4, 6, high half 1, 3, 5, 7.
 //
-// code = rint((x - lo) / scale), halves to the even code, at most 15.  x - lo is exact in fp32 unless a row
-// spans more than 2^13 times its smallest step, so the quotient decides exactly; it costs an IEEE division only
-// where (x - lo) * (1 / scale), which is within 2^-18 of it, lies that near to a half.  Adding 1.5 * 2^23
-// rounds to an integer that then stands in the low mantissa bits.
-__device__ __forceinline__ uint32_t encode8(const float (&x)[8], float lo, float scale) {
+// code = rint((x - lo) / scale), halves to the even code, at most 15, without a division: x - lo is exact in fp32
+// unless a row spans more than 2^13 times its smallest step, and (x - lo) * (1 / scale) is within 2^-18 of the quotient,
+// which decides everything that does not lie that near to a half.  Adding 1.5 * 2^23 in the product's own fma rounds to
+// an integer that then stands in the low mantissa bits, and a second fma gives the distance from it; both, like the
+// differences, two elements at a time.  (scale is max - min over 15 rounded by 2^-9 at most, so nothing exceeds 15.5,
+// unless it is subnormal: `normal` says that it is not.)
+__device__ __forceinline__ void encode16(const float (&x)[16], float lo, float scale, bool normal, uint32_t (&code)[2]) {
     constexpr float kMagic = 12582912.f;
     constexpr uint32_t kMagicBits = 0x4B400000u;
     const float inv = 1.f / scale;
-    uint32_t word = 0;
+    const uint64_t inv2 = pack_f32x2(inv, inv), magic2 = pack_f32x2(kMagic, kMagic), less2 = pack_f32x2(-kMagic, -kMagic),
+                   one2 = pack_f32x2(1.f, 1.f), minus2 = pack_f32x2(-1.f, -1.f), lo2 = pack_f32x2(-lo, -lo);
+    code[0] = code[1] = 0;
     float worst = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float t = fminf((x[j] - lo) * inv, 15.f);
-        const float u = t + kMagic;
-        worst = fmaxf(worst, fabsf(t - (u - kMagic)));
-        word += (__float_as_uint(u) - kMagicBits) << (4 * (j >> 1) + 16 * (j & 1));
+    for (int j = 0; j < 16; j += 2) {
+        const uint64_t d = fma_f32x2(pack_f32x2(x[j], x[j + 1]), one2, lo2);
+        const uint64_t u = fma_f32x2(d, inv2, magic2);
+        const uint64_t r = fma_f32x2(u, one2, less2);
+        const uint64_t e = fma_f32x2(d, inv2, mul_f32x2(r, minus2));
+        float u0, u1, e0, e1;
+        unpack_f32x2(u, u0, u1);
+        unpack_f32x2(e, e0, e1);
+        worst = fmaxf(worst, fmaxf(fabsf(e0), fabsf(e1)));
+        const int k = (j & 7) >> 1;          // nibble of the even element in the low half, of the odd one in the high half
+        code[j >> 3] += ((__float_as_uint(u0) - kMagicBits) << (4 * k)) + ((__float_as_uint(u1) - kMagicBits) << (4 * k + 16));
     }
-    if (worst > 0.5f - 4e-6f || !(inv < INFINITY)) {
-        word = 0;
+    if (!normal) {
+        code[0] = code[1] = 0;
+#pragma unroll 1
+        for (int j = 0; j < 16; ++j) {
+            float v = x[0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float t = fminf(rintf((x[j] - lo) / scale), 15.f);
-            word |= static_cast<uint32_t>(t) << (4 * (j >> 1) + 16 * (j & 1));
+            for (int k = 1; k < 16; ++k) v = j == k ? x[k] : v;
+            const float t = fminf(rintf((v - lo) / scale), 15.f);
+            const uint32_t bits = static_cast<uint32_t>(t) << (4 * ((j & 7) >> 1) + 16 * (j & 1));
+            if (j < 8) code[0] |= bits; else code[1] |= bits;
+        }
+    } else if (worst > 0.5f - 4e-6f) {
+        // Near a half (16-bit numbers meet exact halves often: about every second warp has one): the distance
+        // x - lo - r scale is exact in one fma, and says whether r is the nearest, or which of two to take.
+        code[0] = code[1] = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float d = x[j] - lo, u = fmaf(d, inv, kMagic), rest = fmaf(kMagic - u, scale, d);
+            uint32_t r = __float_as_uint(u) - kMagicBits;
+            const float twice = 2.f * fabsf(rest);
+            if (twice > scale || (twice == scale && (r & 1u))) r += rest > 0.f ? 1u : ~0u;
+            code[j >> 3] |= r << (4 * ((j & 7) >> 1) + 16 * (j & 1));
         }
     }
-    return word;
 }
 
 // D / 16 threads per row (one token, K or V), 16 elements each; the CTA's 32 rows in one or two passes.
@@ -124,134 +168,150 @@ template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) appe
     constexpr int kLanes = D / 16;
     __shared__ __align__(16) unsigned char image[L::kBytes];
     __shared__ TileGroup grp;
-    const int token0 = static_cast<int>(blockIdx.x / p.heads) * 16, head = blockIdx.x % p.heads;
+    const int splits = (p.heads + p.heads_per_cta - 1) / p.heads_per_cta;
+    const int token0 = static_cast<int>(blockIdx.x / splits) * 16;
+    const int head0 = static_cast<int>(blockIdx.x % splits) * p.heads_per_cta, head1 = min(head0 + p.heads_per_cta, p.heads);
     const int row = threadIdx.x / kLanes, i = threadIdx.x % kLanes;
     const int tok_in = row & 15;
     const bool is_v = row >= 16;
     // the rows are requested before the slots are looked at: a padding token's row is read for nothing
-    uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     const bool have = row < 32 && token0 + tok_in < p.num_tokens;
-    if (have) {
-        const int64_t token = token0 + tok_in;
-        const T* src = is_v ? static_cast<const T*>(p.value) + token * p.value_token + head * p.value_head
-                            : static_cast<const T*>(p.key) + token * p.key_token + head * p.key_head;
-        raw[0] = __ldg(reinterpret_cast<const uint4*>(src) + 2 * i);
-        raw[1] = __ldg(reinterpret_cast<const uint4*>(src) + 2 * i + 1);
-    }
-    load_group<D>(p, grp, token0, head);
-    float x[2][8];
-    const uint32_t words[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+    const int64_t token = token0 + tok_in, head_step = is_v ? p.value_head : p.key_head;
+    const T* src = (is_v ? static_cast<const T*>(p.value) + token * p.value_token : static_cast<const T*>(p.key) + token * p.key_token) +
+                   head0 * head_step + 16 * i;
+    uint4 next[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    auto request = [&]() {
+        if (!have) return;
+        next[0] = __ldg(reinterpret_cast<const uint4*>(src));
+        next[1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+        src += head_step;
+    };
+    request();
+    load_group<D>(p, grp, token0);
+#pragma unroll 1
+    for (int head = head0; head < head1; ++head) {
+        const uint32_t words[8] = {next[0].x, next[0].y, next[0].z, next[0].w, next[1].x, next[1].y, next[1].z, next[1].w};
+        if (head + 1 < head1) request();
+        uint32_t lo2 = words[0], hi2 = words[0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float2 e = Int4Elt<T>::unpack(words[j]);
-        x[j >> 2][2 * (j & 3)] = e.x;
-        x[j >> 2][2 * (j & 3) + 1] = e.y;
-    }
-    float lo = x[0][0], hi = x[0][0];
-    bool bad = false;
+        for (int j = 1; j < 8; ++j) min_max_pairs<T>(words[j], lo2, hi2);
+        const float2 lo_pair = Int4Elt<T>::unpack(lo2), hi_pair = Int4Elt<T>::unpack(hi2);
+        float lo = min_or_nan(lo_pair.x, lo_pair.y), hi = max_or_nan(hi_pair.x, hi_pair.y);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const float v = x[j >> 3][j & 7];
-        lo = fminf(lo, v);
-        hi = fmaxf(hi, v);
-        bad = bad || !(fabsf(v) <= FLT_MAX);
-    }
-#pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(kFullMask, lo, d));
-        hi = fmaxf(hi, __shfl_xor_sync(kFullMask, hi, d));
-    }
-    const uint32_t bad_lanes = __ballot_sync(kFullMask, bad);
-    bad = ((bad_lanes >> (threadIdx.x & 31 & ~(kLanes - 1))) & ((1u << kLanes) - 1u)) != 0;
-    float scale;
-    if (hi - lo <= FLT_MAX) {
-        scale = elt_round<T>((hi - lo) / 15.f);
-    } else {                   // a bf16 row may span more than fp32 can hold: everything halved, which is exact
-        scale = elt_round<T>((0.5f * hi - 0.5f * lo) / 7.5f);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j >> 3][j & 7] *= 0.5f;
-    }
-    if (bad) scale = NAN;
-    const float half = hi - lo <= FLT_MAX ? 1.f : 0.5f;
-    const uint32_t prm = Elt<T>::pack(scale, bad ? NAN : lo);
-    uint32_t code[2] = {0, 0};
-    if (scale > 0.f) {
-        code[0] = encode8(x[0], half * lo, half * scale);
-        code[1] = encode8(x[1], half * lo, half * scale);
-    }
-    // where the row goes: the image of the tile, or straight to the cache
-    unsigned char* tile = image;
-    int tok = tok_in;
-    if (!grp.tile) {
-        const int64_t slot = grp.slot[tok_in];
-        tile = have && slot >= 0 ? tile_of_slot<D>(p, slot, head, tok) : nullptr;
-    }
-    if (tile && row < 32) {
-        if (!is_v) {
-            *reinterpret_cast<uint2*>(tile + k_word_off<D>(tok, 2 * i)) = make_uint2(code[0], code[1]);
-        } else {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                uint16_t* dst = reinterpret_cast<uint16_t*>(tile + v_half_off<D>(tok, 2 * i + b));
-                dst[0] = static_cast<uint16_t>(code[b]);
-                dst[2] = static_cast<uint16_t>(code[b] >> 16);
-            }
+        for (int d = kLanes / 2; d > 0; d >>= 1) {
+            lo = min_or_nan(lo, __shfl_xor_sync(kFullMask, lo, d));
+            hi = max_or_nan(hi, __shfl_xor_sync(kFullMask, hi, d));
         }
-        if (i == 0) *reinterpret_cast<uint32_t*>(tile + (is_v ? L::kVPrm : L::kKPrm) + tok * 4) = prm;
-    }
-    if (grp.tile) {
-        __syncthreads();
-        for (int j = threadIdx.x; j < L::kBytes / 16; j += kRowThreads)
-            reinterpret_cast<uint4*>(grp.tile)[j] = reinterpret_cast<const uint4*>(image)[j];
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 e = Int4Elt<T>::unpack(words[j]);
+            x[2 * j] = e.x;
+            x[2 * j + 1] = e.y;
+        }
+        const bool bad = !(fabsf(lo) <= FLT_MAX && fabsf(hi) <= FLT_MAX);
+        float scale, half = 1.f;
+        if (bad || hi - lo <= FLT_MAX) {
+            scale = elt_round<T>((hi - lo) / 15.f);
+        } else {                   // a bf16 row may span more than fp32 can hold: everything halved, which is exact
+            scale = elt_round<T>((0.5f * hi - 0.5f * lo) / 7.5f);
+            half = 0.5f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] *= 0.5f;
+        }
+        if (bad) scale = NAN;
+        const uint32_t prm = Elt<T>::pack(scale, bad ? NAN : lo);
+        uint32_t code[2] = {0, 0};
+        constexpr float kNormal = Int4Elt<T>::kIsHalf ? 6.103515625e-05f : 2.35098870164457501594e-38f;    // (bf16: a reciprocal stays finite)
+        if (scale > 0.f) encode16(x, half * lo, half * scale, scale >= kNormal, code);
+        // where the row goes: the image of the tile, or straight to the cache
+        unsigned char* tile = image;
+        int tok = tok_in;
+        if (!grp.tile) {
+            const int64_t slot = grp.slot[tok_in];
+            tile = have && slot >= 0 ? tile_of_slot<D>(p, slot, head, tok) : nullptr;
+        }
+        if (tile && row < 32) {
+            if (!is_v) {
+                *reinterpret_cast<uint2*>(tile + k_word_off<D>(tok, 2 * i)) = make_uint2(code[0], code[1]);
+            } else {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    uint16_t* dst = reinterpret_cast<uint16_t*>(tile + v_half_off<D>(tok, 2 * i + b));
+                    dst[0] = static_cast<uint16_t>(code[b]);
+                    dst[2] = static_cast<uint16_t>(code[b] >> 16);
+                }
+            }
+            if (i == 0) *reinterpret_cast<uint32_t*>(tile + (is_v ? L::kVPrm : L::kKPrm) + tok * 4) = prm;
+        }
+        if (grp.tile) {
+            __syncthreads();
+            for (int j = threadIdx.x; j < L::kBytes / 16; j += kRowThreads)
+                reinterpret_cast<uint4*>(grp.tile + head * p.head_stride)[j] = reinterpret_cast<const uint4*>(image)[j];
+            __syncthreads();
+        }
     }
 }
 
 // The inverse: value = lo + scale * code in fp32 (one rounding, the product is exact), rounded to T.
 // D / 8 threads per row, 8 elements each.
-template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) gather_int4_kernel(const RowsParams p) {
+template <typename T, int D> __global__ void __launch_bounds__(kRowThreads, 8) gather_int4_kernel(const RowsParams p) {
     using L = Int4Tile<D>;
     constexpr int kLanes = D / 8, kRowsPerPass = kRowThreads / kLanes;
     __shared__ __align__(16) unsigned char image[L::kBytes];
     __shared__ TileGroup grp;
-    const int token0 = static_cast<int>(blockIdx.x / p.heads) * 16, head = blockIdx.x % p.heads;
-    load_group<D>(p, grp, token0, head);
-    if (grp.tile) {
-        for (int j = threadIdx.x; j < L::kBytes / 16; j += kRowThreads)
-            reinterpret_cast<uint4*>(image)[j] = __ldg(reinterpret_cast<const uint4*>(grp.tile) + j);
-        __syncthreads();
-    }
+    const int splits = (p.heads + p.heads_per_cta - 1) / p.heads_per_cta;
+    const int token0 = static_cast<int>(blockIdx.x / splits) * 16;
+    const int head0 = static_cast<int>(blockIdx.x % splits) * p.heads_per_cta, head1 = min(head0 + p.heads_per_cta, p.heads);
+    load_group<D>(p, grp, token0);
+    constexpr int kVecs = L::kBytes / 16;
+    static_assert(kVecs <= kRowThreads, "one 16-byte piece of a tile per thread");
+    uint4 next = make_uint4(0, 0, 0, 0);
     const int i = threadIdx.x % kLanes;
+    if (grp.tile && threadIdx.x < kVecs) next = __ldg(reinterpret_cast<const uint4*>(grp.tile + head0 * p.head_stride) + threadIdx.x);
+#pragma unroll 1
+    for (int head = head0; head < head1; ++head) {
+        if (grp.tile) {
+            if (threadIdx.x < kVecs) {
+                reinterpret_cast<uint4*>(image)[threadIdx.x] = next;
+                if (head + 1 < head1) next = __ldg(reinterpret_cast<const uint4*>(grp.tile + (head + 1) * p.head_stride) + threadIdx.x);
+            }
+            __syncthreads();
+        }
 #pragma unroll
-    for (int row = threadIdx.x / kLanes; row < 32; row += kRowsPerPass) {
-        const int tok_in = row & 15;
-        const bool is_v = row >= 16;
-        const unsigned char* tile = image;
-        int tok = tok_in;
-        if (!grp.tile) {
-            const int64_t slot = grp.slot[tok_in];
-            if (slot < 0) continue;
-            tile = tile_of_slot<D>(p, slot, head, tok);
-        }
-        uint32_t word;
-        if (!is_v) {
-            word = *reinterpret_cast<const uint32_t*>(tile + k_word_off<D>(tok, i));
-        } else {
-            const uint16_t* src = reinterpret_cast<const uint16_t*>(tile + v_half_off<D>(tok, i));
-            word = src[0] | (static_cast<uint32_t>(src[2]) << 16);
-        }
-        const float2 prm = Int4Elt<T>::unpack(*reinterpret_cast<const uint32_t*>(tile + (is_v ? L::kVPrm : L::kKPrm) + tok * 4));
-        const uint32_t pairs[4] = {Int4Elt<T>::template pair<0>(word), Int4Elt<T>::template pair<1>(word),
-                                   Int4Elt<T>::template pair<2>(word), Int4Elt<T>::template pair<3>(word)};
-        uint32_t out[4];
+        for (int r = 0; r < 32 / kRowsPerPass; ++r) {
+            const int row = threadIdx.x / kLanes + r * kRowsPerPass;
+            const int tok_in = row & 15;
+            const bool is_v = row >= 16;
+            const unsigned char* tile = image;
+            int tok = tok_in;
+            if (!grp.tile) {
+                const int64_t slot = grp.slot[tok_in];
+                if (slot < 0) continue;
+                tile = tile_of_slot<D>(p, slot, head, tok);
+            }
+            uint32_t word;
+            if (!is_v) {
+                word = *reinterpret_cast<const uint32_t*>(tile + k_word_off<D>(tok, i));
+            } else {
+                const uint16_t* src = reinterpret_cast<const uint16_t*>(tile + v_half_off<D>(tok, i));
+                word = src[0] | (static_cast<uint32_t>(src[2]) << 16);
+            }
+            const float2 prm = Int4Elt<T>::unpack(*reinterpret_cast<const uint32_t*>(tile + (is_v ? L::kVPrm : L::kKPrm) + tok * 4));
+            const uint32_t pairs[4] = {Int4Elt<T>::template pair<0>(word), Int4Elt<T>::template pair<1>(word),
+                                       Int4Elt<T>::template pair<2>(word), Int4Elt<T>::template pair<3>(word)};
+            uint32_t out[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 c = Int4Elt<T>::unpack(pairs[j]);       // 16 + code
-            out[j] = Elt<T>::pack(fmaf(c.x - 16.f, prm.x, prm.y), fmaf(c.y - 16.f, prm.x, prm.y));
+            for (int j = 0; j < 4; ++j) {
+                const float2 c = Int4Elt<T>::unpack(pairs[j]);       // 16 + code
+                out[j] = Elt<T>::pack(fmaf(c.x - 16.f, prm.x, prm.y), fmaf(c.y - 16.f, prm.x, prm.y));
+            }
+            const int64_t token = token0 + tok_in;
+            T* dst = is_v ? static_cast<T*>(p.value) + token * p.value_token + head * p.value_head
+                          : static_cast<T*>(p.key) + token * p.key_token + head * p.key_head;
+            reinterpret_cast<uint4*>(dst)[i] = make_uint4(out[0], out[1], out[2], out[3]);
         }
-        const int64_t token = token0 + tok_in;
-        T* dst = is_v ? static_cast<T*>(p.value) + token * p.value_token + head * p.value_head
-                      : static_cast<T*>(p.key) + token * p.key_token + head * p.key_head;
-        reinterpret_cast<uint4*>(dst)[i] = make_uint4(out[0], out[1], out[2], out[3]);
+        if (grp.tile) __syncthreads();
     }
 }
 
@@ -270,7 +330,18 @@ int check_device(int* dev) {
     return PAT_OK;
 }
 
-int64_t row_blocks(const pat_int4_rows_args& a) { return (static_cast<int64_t>(a.num_tokens) + 15) / 16 * a.num_kv_heads; }
+// KV heads per CTA: with a CTA for each of them (head by head) a short call fills more SMs; a long one is faster when a
+// CTA walks the heads of its tokens, since it then waits for memory once.  Half a wave of 8 CTAs per SM divides the two.
+int heads_per_cta(const pat_int4_rows_args& a) {
+    const int64_t groups = (static_cast<int64_t>(a.num_tokens) + 15) / 16;
+    int n = 1;
+    while (n < a.num_kv_heads && groups * ((a.num_kv_heads + 2 * n - 1) / (2 * n)) >= 4 * 148) n *= 2;
+    return n;
+}
+int64_t row_blocks(const pat_int4_rows_args& a) {
+    const int n = heads_per_cta(a);
+    return (static_cast<int64_t>(a.num_tokens) + 15) / 16 * ((a.num_kv_heads + n - 1) / n);
+}
 
 int rows_params(const pat_int4_rows_args& a, RowsParams* out) {
     if (a.num_tokens < 0 || a.num_kv_heads <= 0 || a.num_pages <= 0) return PAT_ERR_BAD_ARGUMENT;
@@ -299,6 +370,7 @@ int rows_params(const pat_int4_rows_args& a, RowsParams* out) {
     p.num_tokens = a.num_tokens;
     p.heads = a.num_kv_heads;
     p.page_size = a.page_size;
+    p.heads_per_cta = heads_per_cta(a);
     if (row_blocks(a) > 0x7fffffffLL || a.num_tokens > 0x7fffffff - 16) return PAT_ERR_TOO_LARGE;
     *out = p;
     return PAT_OK;
