@@ -403,7 +403,7 @@ template <typename T, int D> int launch_attention(const pat_decode_int4_args& a,
     p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
     p.status = a.status_word;
     p.wait_ns = a.wait_limit_us > 0 ? static_cast<uint64_t>(a.wait_limit_us) * 1000ull : kDefaultWaitNs;
-    const Int4Cache cache{static_cast<const unsigned char*>(a.kv_cache), a.page_stride, a.head_stride};
+    const Int4Cache cache{static_cast<const unsigned char*>(a.kv_cache), a.page_stride, a.head_stride, 64u};
 
     // The order of the 16-bit path: dense kernel, streaming kernel as its programmatic dependent, merge (which
     // waits for the last dense CTA through a control word of the workspace).

@@ -35,12 +35,17 @@ template <int D> struct Int4Tile {
 // count ones when the exponent says 16 (bits 3-6 of bf16, bits 6-9 of fp16).  Exact, one shift and
 // one logic instruction per pair; the constant 16 is taken out of the sums in fp32.
 template <typename T> struct Int4Elt;
+template <uint32_t kMask> __device__ __forceinline__ uint32_t mask_or(uint32_t v, uint32_t bits) {       // (v & kMask) | bits
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "n"(kMask), "r"(bits));
+    return r;
+}
 template <> struct Int4Elt<__nv_bfloat16> {
     static constexpr bool kIsHalf = false;
     static constexpr uint32_t kSixteen = 0x41804180u;     // (16, 16)
     template <int J> __device__ static __forceinline__ uint32_t pair(uint32_t w) {
         const uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3);
-        return (x & 0x00780078u) | kSixteen;
+        return mask_or<0x00780078u>(x, kSixteen);
     }
     __device__ static __forceinline__ float2 unpack(uint32_t v) {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
@@ -51,7 +56,7 @@ template <> struct Int4Elt<__half> {
     static constexpr uint32_t kSixteen = 0x4C004C00u;
     template <int J> __device__ static __forceinline__ uint32_t pair(uint32_t w) {
         const uint32_t x = J < 2 ? w << (6 - 4 * J) : w >> (4 * J - 6);
-        return (x & 0x03C003C0u) | kSixteen;
+        return mask_or<0x03C003C0u>(x, kSixteen);
     }
     __device__ static __forceinline__ float2 unpack(uint32_t v) {
         return __half22float2(*reinterpret_cast<const __half2*>(&v));
@@ -81,6 +86,7 @@ template <int N> __device__ __forceinline__ void lds_words(uint32_t (&w)[N], con
 struct Int4Cache {
     const unsigned char* base;
     int64_t page_stride, head_stride;      // bytes
+    uint32_t sixty_four;                   // 64 (see Codes16)
 };
 
 // A warp works off one unit - a streaming item's rows (8 or fewer) of one KV head - by itself: no barrier, nothing to
@@ -96,17 +102,18 @@ template <int D> constexpr int int4_stream_smem_bytes() {
 
 // The streaming kernel multiplies in fp16 whatever the model's type.  fp16 has ten mantissa bits, so two of a word's
 // nibbles become numbers without being moved: under the exponent of 64 the bits 4-7 count ones (64 + c); bits 0-3 are
-// moved to 6-9, under the exponent of 16 (16 + c).  A word costs one shift, four logic instructions and two
-// multiplications by 64 (which run on the fma pipe: the integer pipe, at half rate, bounds this kernel) where bf16 takes
-// four shifts and four logic instructions, and P' keeps eleven bits instead of eight.
+// moved to 6-9, under the exponent of 16 (16 + c).  A word costs one shift, four logic instructions (mask and
+// exponent in one three-input instruction each) and two multiplications by 64, where bf16 takes four shifts and four
+// logic instructions, and P' keeps eleven bits instead of eight.  The integer pipe, at half rate, bounds this kernel: the
+// factor 64 is a kernel parameter because a multiplication by a constant would become a shift on that pipe.
 struct Codes16 {
     uint32_t p[4];                         // pairs of nibble 0 .. 3: 16 + c, 64 + c, 16 + c, 64 + c
-    __device__ __forceinline__ explicit Codes16(uint32_t w) {
+    __device__ __forceinline__ Codes16(uint32_t w, uint32_t sixty_four) {
         const uint32_t w8 = w >> 8;
-        p[0] = ((w * 64u) & 0x03C003C0u) | 0x4C004C00u;
-        p[1] = (w & 0x00F000F0u) | 0x54005400u;
-        p[2] = ((w8 * 64u) & 0x03C003C0u) | 0x4C004C00u;
-        p[3] = (w8 & 0x00F000F0u) | 0x54005400u;
+        p[0] = mask_or<0x03C003C0u>(w * sixty_four, 0x4C004C00u);
+        p[1] = mask_or<0x00F000F0u>(w, 0x54005400u);
+        p[2] = mask_or<0x03C003C0u>(w8 * sixty_four, 0x4C004C00u);
+        p[3] = mask_or<0x00F000F0u>(w8, 0x54005400u);
     }
 };
 constexpr float kInt4NormStart = 1.329227995784916e36f;     // 2^120: any scale but the tiniest exceeds 1 / this
@@ -143,7 +150,8 @@ template <int D> struct Int4State {
 // fp16 has too few exponents for p * s of any s: s is taken relative to 1 / `vnorm`, a power of two near the
 // largest scale seen.
 template <typename T, int D, bool kLimits>
-__device__ __forceinline__ void int4_attend_step(Int4State<D>& st, const unsigned char* stage, int valid, int lim0, int lim1, int lane) {
+__device__ __forceinline__ void int4_attend_step(Int4State<D>& st, const unsigned char* stage, int valid, int lim0, int lim1, uint32_t k64,
+                                                 int lane) {
     using E = Int4Elt<T>;
     using H = Elt<__half>;
     using L = Int4Tile<D>;
@@ -161,7 +169,7 @@ __device__ __forceinline__ void int4_attend_step(Int4State<D>& st, const unsigne
         x[u][1] = x[u][3] = st.qoff[1];
 #pragma unroll
         for (int w = 0; w < W4; ++w) {
-            const Codes16 f0(k0[w]), f1(k1[w]);
+            const Codes16 f0(k0[w], k64), f1(k1[w], k64);
             const uint32_t a[4] = {f0.p[0], f1.p[0], f0.p[1], f1.p[1]};
             const uint32_t b[4] = {f0.p[2], f1.p[2], f0.p[3], f1.p[3]};
             H::mma(x[u], a, st.q[2 * w].x, st.q[2 * w].y);
@@ -261,7 +269,7 @@ __device__ __forceinline__ void int4_attend_step(Int4State<D>& st, const unsigne
         H::mma(st.off, ones, pb0, pb1);
 #pragma unroll
         for (int wp = 0; wp < D / 64; ++wp) {
-            const Codes16 a0(v0[2 * wp]), a1(v0[2 * wp + 1]), a2(v1[2 * wp]), a3(v1[2 * wp + 1]);
+            const Codes16 a0(v0[2 * wp], k64), a1(v0[2 * wp + 1], k64), a2(v1[2 * wp], k64), a3(v1[2 * wp + 1], k64);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t f[4] = {a0.p[j], a1.p[j], a2.p[j], a3.p[j]};
@@ -418,7 +426,8 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 4) int4_stream_kernel(const A
                 if (lane == 0 && p.status) atomicExch(p.status, 1);
                 return;
             }
-            int4_attend_step<T, D, kLimits>(st, my_stage + s * kStage, kv_len - j * 16 * U, lim[0] - j * 16 * U, lim[1] - j * 16 * U, lane);
+            int4_attend_step<T, D, kLimits>(st, my_stage + s * kStage, kv_len - j * 16 * U, lim[0] - j * 16 * U, lim[1] - j * 16 * U,
+                                            cache.sixty_four, lane);
             __syncwarp();
             if ((j + S) % kAhead == 0) fetch(j + S);
             if (j + S < n_steps) issue(j + S);
