@@ -944,9 +944,19 @@ def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree,
         work = info.device_work(q.device, int4_config(), q.shape[1])
         known = info._int4_calls.remember(sig, (work, *_int4_tail(q, kv_cache, work, out, softmax_scale, _flags, _wait_limit_us)))
     work, need, tail = known
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return prefix_attn_with_int4_kvcache(q, kv_cache, tree, softmax_scale, out, lse_out, _status=_status, _flags=_flags,
+                                                 _wait_limit_us=_wait_limit_us)
     stream = torch._C._cuda_getCurrentRawStream(index)
     ws = work._scratch.get(stream)
-    if stream != work._upload_stream or ws is None or ws.numel() < need:
+    if torch.cuda.is_current_stream_capturing():
+        # A workspace of the graph's own: graphs captured on one stream may be replayed on several.  Its control words
+        # are cleared in the graph where kernels run beside each other and use them.
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        if work.header.num_stream_items and work.header.num_dense_items:
+            ws[:_WS_HEAD].zero_()
+    elif stream != work._upload_stream or ws is None or ws.numel() < need:
         current = torch.cuda.current_stream(index)
         work.order_after_upload(current)
         ws = work.workspace(need, current, q.device)

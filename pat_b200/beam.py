@@ -39,19 +39,29 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int, finish
     known = _beam_calls.get(sig)
     if known is None:
         known = _beam_calls.remember(sig, _check_beam(logits, scores, num_out, finished, pad_token))
-    tail, index, shape, need, dense_scores, dense_finished = known
+    tail, index, batch, num_out, need, dense_scores, dense_finished = known
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return beam_select(logits, scores, num_out, finished, pad_token)
     dev = logits.device
-    out_scores = torch.empty(shape, dtype=torch.float32, device=dev)
-    out_parents = torch.empty(shape, dtype=torch.int32, device=dev)
-    out_tokens = torch.empty(shape, dtype=torch.int32, device=dev)
-    if shape[0] == 0:
+    out_scores = torch.empty(batch, num_out, dtype=torch.float32, device=dev)
+    out_parents = torch.empty(batch, num_out, dtype=torch.int32, device=dev)
+    out_tokens = torch.empty(batch, num_out, dtype=torch.int32, device=dev)
+    if batch == 0:
         return out_scores, out_parents, out_tokens
     if not dense_scores:
         scores = scores.contiguous()
     if not dense_finished:
         finished = finished.contiguous()
-    # (scratch of this call alone; inside a stream capture it belongs to the graph)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    # Scratch: calls on one stream run one after the other and share it; a captured call gets its own, which belongs to
+    # the graph, since graphs captured on one stream may be replayed on several.
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        key = (index, torch._C._cuda_getCurrentRawStream(index))
+        ws = _beam_scratch.get(key)
+        if ws is None or ws.numel() < need:
+            ws = _beam_scratch[key] = torch.empty(need, dtype=torch.uint8, device=dev)
     rc = launch(N.load().pat_b200_beam_select,
                 _BEAM_POINTERS.pack(logits.data_ptr(), scores.data_ptr(), finished.data_ptr() if finished is not None else 0,
                                     out_scores.data_ptr(), out_parents.data_ptr(), out_tokens.data_ptr(), ws.data_ptr()) + tail, index)
@@ -62,6 +72,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int, finish
 
 _BEAM_POINTERS = struct.Struct("7P")
 _beam_calls = Signatures()
+_beam_scratch = {}         # (device, stream) -> workspace
 
 
 def _check_beam(logits, scores, num_out, finished, pad_token):
@@ -101,7 +112,7 @@ def _check_beam(logits, scores, num_out, finished, pad_token):
     a.batch, a.beams, a.vocab, a.num_out = batch, beams, vocab, int(num_out)
     a.dtype, a.pad_token = _LOGIT_DTYPES[logits.dtype], int(pad_token)
     a.workspace_bytes = need
-    return struct_tail(a, _BEAM_POINTERS.size), logits.get_device(), (batch, int(num_out)), need, dense_scores, dense_finished
+    return struct_tail(a, _BEAM_POINTERS.size), logits.get_device(), batch, int(num_out), need, dense_scores, dense_finished
 
 
 class PagePool:

@@ -551,6 +551,42 @@ def test_streams_graphs_and_growing_batches(native_lib):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["lengths", "shared", "tree"])
+def test_two_graphs_of_one_plan_replayed_at_once(kind, native_lib):
+    """Both were captured on the same stream; each has a workspace of its own."""
+    page, hq, hk, d = 16, 16, 2, 128
+    lens, tables, pages = _batch(kind, page, 8)
+    cache = _fill(pages, page, hk, d, BF16, 4)
+    tree = _tree(lens, tables, page, hq // hk, hk)
+    g = torch.Generator().manual_seed(5)
+    qs = [(torch.randn(len(lens), 1, hq, d, generator=g) * 0.5).to(BF16).to(DEV) for _ in range(2)]
+    want, graphs = [], []
+    for q in qs:
+        out = torch.empty_like(q)
+        prefix_attn_with_int4_kvcache(q, cache, tree, 0.09, out)
+        want.append(out)
+    torch.cuda.synchronize()
+    for q in qs:
+        out = torch.empty_like(q)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            prefix_attn_with_int4_kvcache(q, cache, tree, 0.09, out)
+        graphs.append((gr, out))
+    for _ in range(3):
+        for _, out in graphs:
+            out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(4):
+            for (gr, _), st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    gr.replay()
+        torch.cuda.synchronize()
+        for (_, out), w in zip(graphs, want):
+            assert torch.equal(out, w)
+
+
+@gpu
 def test_append_then_attend(native_lib):
     """A decode step: append the new token of every request, attend over the context that includes it; the
     attention over 4 bits is the 16-bit one over the rows the cache stands for."""
