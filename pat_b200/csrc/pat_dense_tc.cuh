@@ -64,9 +64,7 @@ constexpr float kTcLazyLog2 = 8.0f;
 template <int D, bool kInt4> struct TcSmem {
     static constexpr int kBoxes = D / 64;
     static constexpr int kKvRing = kInt4 ? 2 : kTcRing;
-    // A granule is loaded once the one six before it has been unpacked, whose V slot was free: eight tiles back everything
-    // is done, whatever the tiles' lengths, and the parameters of a tile (kPrmRing) may replace those of that one.
-    static constexpr int kRawRing = 6, kPrmRing = 8;
+    static constexpr int kPrmRing = 4, kRawRing = 7;
     static constexpr int kRawBytes = 4 * Int4Tile<D>::kBytes;
     static constexpr int kQBytes = kBoxes * 128 * 128;          // [box][128 rows][128 B]
     static constexpr int kKBytes = kBoxes * kTcTile * 128;      // [box][128 tokens][128 B]
@@ -74,7 +72,7 @@ template <int D, bool kInt4> struct TcSmem {
     static constexpr int kKOff = kQOff + kQBytes;               // K ring
     static constexpr int kVOff = kKOff + kKvRing * kKBytes;     // V ring
     static constexpr int kRawOff = kVOff + kKvRing * kKBytes;
-    static constexpr int kBarOff = kRawOff + (kInt4 ? kRawRing * kRawBytes : 0);    // 43 mbarriers (kInt4: 63) + tmem base word + flag
+    static constexpr int kBarOff = kRawOff + (kInt4 ? kRawRing * kRawBytes : 0);    // 43 mbarriers (kInt4: 61) + tmem base word + flag
     static constexpr int kXchOff = kBarOff + 512;               // float[2][2][128]: row maxima / sums of the two column halves
     static constexpr int kPrmOff = kXchOff + 2048;              // kInt4: float[ring][2][128], factor and addend of every token's scores
     static constexpr int kRequest = kPrmOff + (kInt4 ? kPrmRing * 1024 : 0);
@@ -298,11 +296,10 @@ template <typename T> __device__ __forceinline__ bool params_are_finite(uint32_t
     return (prm & e) != e && (prm >> 16 & e) != e;
 }
 
-// The warp that requests the raw granules, page ids fetched a granule ahead of the request that needs them.  It also
-// writes down, for every token, what turns the products of its codes into scores.
+// The warp that requests the raw granules.  Page ids are fetched a granule ahead of the request that needs them.
 template <typename T, int D>
 __device__ __forceinline__ void load_granules(const DenseTcParams& dp, const Int4Cache& cache, int lane, int item_lo, int item_hi,
-                                              const unsigned char* raw, uint32_t bar_raw, float* prm, uint32_t bar_prm) {
+                                              uint32_t raw, uint32_t bar_raw) {
     using L = TcSmem<D, true>;
     using I = Int4Tile<D>;
     constexpr int RR = L::kRawRing;
@@ -342,40 +339,6 @@ __device__ __forceinline__ void load_granules(const DenseTcParams& dp, const Int
     bool ok = true;
     int n = 0, slot = 0;
     uint32_t phase = 1;                     // parity of the release that precedes the current use of the slot
-    // the granule whose parameters come next: its item, first token, tile and place in the ring
-    int at_item = item_lo, at_tok = 0, at_t = 0, at_n = 0, at_slot = 0;
-    uint32_t at_phase = 0;
-    auto parameters = [&]() {
-        ok = __all_sync(kFullMask, mbar_wait_in<true>(raw_full + 8 * at_slot, at_phase, p.wait_ns));
-        if (!ok) return;
-        const int kv_len = __ldg(p.items + static_cast<size_t>(at_item) * 8 + 3);
-        float* out = prm + (at_t % L::kPrmRing) * 256 + (at_tok & 64);
-        const int left = kv_len - at_tok;           // tokens from this granule's first on
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int tok = lane + 32 * e;
-            const unsigned char* src = raw + at_slot * L::kRawBytes + (tok >> 4) * I::kBytes + (tok & 15) * 4;
-            float factor = 0.f, addend = 0.f;       // tokens past the end
-            if (tok < left) {
-                const float2 kp = Int4Elt<T>::unpack(*reinterpret_cast<const uint32_t*>(src + I::kKPrm));
-                factor = kp.x * p.scale_log2;
-                addend = params_are_finite<T>(*reinterpret_cast<const uint32_t*>(src + I::kVPrm)) ? (kp.y - 16.f * kp.x) * p.scale_log2 : NAN;
-            }
-            out[tok] = factor;
-            out[128 + tok] = addend;
-            if (!(at_tok & 64) && left <= 64) out[64 + tok] = out[192 + tok] = 0.f;       // the tile has no second granule
-        }
-        __syncwarp();
-        if (lane == 0) {
-            mbar_arrive(raw_empty + 8 * at_slot);
-            if ((at_tok & 64) || left <= 64) mbar_arrive(bar_prm + 8 * (at_t % L::kPrmRing));
-        }
-        if ((at_tok & 64) || left <= 64) ++at_t;
-        ++at_n;
-        if (++at_slot == RR) { at_slot = 0; at_phase ^= 1; }
-        at_tok += 64;
-        if (left <= 64) { ++at_item; at_tok = 0; }
-    };
     look_up();
     while (subs > 0) {
         const int now = subs, now_in_page = in_page, now_kvh = kvh;
@@ -386,15 +349,12 @@ __device__ __forceinline__ void load_granules(const DenseTcParams& dp, const Int
         if (lane == 0) mbar_expect_tx(raw_full + 8 * slot, now * I::kBytes);
         __syncwarp();
         if (lane < now)
-            bulk_load(smem_u32(raw) + slot * L::kRawBytes + lane * I::kBytes,
+            bulk_load(raw + slot * L::kRawBytes + lane * I::kBytes,
                       cache.base + now_page * cache.page_stride + now_kvh * cache.head_stride + now_in_page * I::kBytes, I::kBytes,
                       raw_full + 8 * slot);
         ++n;
         if (++slot == RR) { slot = 0; phase ^= 1; }
-        if (n - at_n >= 3) parameters();        // (by now it has landed)
-        if (!ok) break;
     }
-    while (ok && at_n < n) parameters();
     if (!ok) {
         // Gave up: nothing more is requested; granules still on their way get a short second wait so that none lands
         // after the CTA has handed its shared memory back.
@@ -407,7 +367,8 @@ __device__ __forceinline__ void load_granules(const DenseTcParams& dp, const Int
 // warps of a group.
 template <typename T, int D, bool kV>
 __device__ __forceinline__ void unpack_operand(const DenseTcParams& dp, int who, int lane, int item_lo, int item_hi, uint32_t ring,
-                                               const unsigned char* raw, uint32_t bar_full, uint32_t bar_empty, uint32_t bar_raw) {
+                                               const unsigned char* raw, uint32_t bar_full, uint32_t bar_empty, uint32_t bar_raw,
+                                               float* prm, uint32_t bar_prm) {
     using L = TcSmem<D, true>;
     using I = Int4Tile<D>;
     constexpr int kWords = D / 32, kGroup = kV ? kTcUnpackV : kTcUnpackK, kRing = L::kKvRing, RR = L::kRawRing;
@@ -448,6 +409,20 @@ __device__ __forceinline__ void unpack_operand(const DenseTcParams& dp, int who,
                 if (loaded && ok) ok = __all_sync(kFullMask, mbar_wait_in<true>(raw_full + 8 * rs, raw_phase, p.wait_ns));
                 if (!ok) break;
                 const unsigned char* rt = raw + rs * L::kRawBytes;
+                if constexpr (!kV) {            // a token a lane: what turns its products into scores
+                    static_assert(kTcUnpackK == 2, "32 of a granule's tokens per warp");
+                    const int tok = lane + 32 * who, row = half * 64 + tok;
+                    const unsigned char* src = rt + (tok >> 4) * I::kBytes + (tok & 15) * 4;
+                    float factor = 0.f, addend = 0.f;
+                    if (row < valid) {
+                        const float2 kp = Int4Elt<T>::unpack(*reinterpret_cast<const uint32_t*>(src + I::kKPrm));
+                        factor = kp.x * p.scale_log2;
+                        addend = params_are_finite<T>(*reinterpret_cast<const uint32_t*>(src + I::kVPrm))
+                                     ? (kp.y - 16.f * kp.x) * p.scale_log2 : NAN;
+                    }
+                    prm[(t & 3) * 256 + row] = factor;
+                    prm[(t & 3) * 256 + 128 + row] = addend;
+                }
 #pragma unroll 1
                 for (int u = who; u < 4; u += kGroup) {         // 16 tokens, as two units whose arithmetic interleaves
                     const unsigned char* src = rt + u * I::kBytes;
@@ -503,7 +478,12 @@ __device__ __forceinline__ void unpack_operand(const DenseTcParams& dp, int who,
             if (!ok) break;
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_full + 8 * slot);
+            if (lane == 0) {
+                mbar_arrive(bar_full + 8 * slot);
+                // (The next use of a parameter slot, four tiles on, waits for the product of tile t + 2, which is
+                // requested after the P V of tile t and so after that tile's softmax.)
+                if (!kV) mbar_arrive(bar_prm + 8 * (t & 3));
+            }
             if (++slot == kRing) { slot = 0; free_phase ^= 1; }
         }
     }
@@ -546,7 +526,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
         return;
     }
     const uint32_t sQ = base + L::kQOff, sK = base + L::kKOff, sV = base + L::kVOff;
-    const uint32_t bars = base + L::kBarOff;
+    const uint32_t bars = base + L::kBarOff, sRaw = base + L::kRawOff;
     // barrier map (8 bytes each): full_k[R] empty_k[R] full_v[R] empty_v[R] s_full[R] p_ready[R]
     // o_done[R] q_ready o_free drain
     const uint32_t bar_full_k = bars, bar_empty_k = bars + 8 * R, bar_full_v = bars + 16 * R, bar_empty_v = bars + 24 * R,
@@ -554,7 +534,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
                    bar_ofree = bars + 56 * R + 8, bar_drain = bars + 56 * R + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tc_smem + L::kBarOff + 56 * R + 24);
     volatile int* poisoned = reinterpret_cast<volatile int*>(tc_smem + L::kBarOff + 56 * R + 32);
-    const uint32_t bar_prm = bars + 56 * R + 40, bar_raw = bar_prm + 8 * L::kPrmRing;      // kInt4: [8]; full [6], empty [6]
+    const uint32_t bar_prm = bars + 56 * R + 40, bar_raw = bar_prm + 32;        // kInt4: [4]; full [7], empty [7]
     float* xch = reinterpret_cast<float*>(tc_smem + L::kXchOff);      // [2][2][128]
 
     // If an earlier CTA of this call already gave up on a wait, do not start (uniform decision).
@@ -575,7 +555,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
             mbar_init(bar_full_k + 8 * i, !kInt4 ? 1 : i / R == 0 ? kTcUnpackK : i / R == 2 ? kTcUnpackV : 1);
         if constexpr (kInt4)
             for (int i = 0; i < L::kPrmRing + 2 * L::kRawRing; ++i)
-                mbar_init(bar_prm + 8 * i, i < L::kPrmRing + L::kRawRing ? 1 : kTcUnpackWarps + 1);
+                mbar_init(bar_prm + 8 * i, i < L::kPrmRing ? kTcUnpackK : i < L::kPrmRing + L::kRawRing ? 1 : kTcUnpackWarps);
         for (int i = 0; i < R; ++i) mbar_init(bar_p + 8 * i, kSW * 32);         // p_ready: every softmax thread
         for (int i = 0; i < R; ++i) mbar_init(bar_o + 8 * i, 1);                // o_done
         mbar_init(bar_q, kSW * 32);                                             // q_ready
@@ -598,12 +578,13 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
             const int who = warp - kSW - 2;                         // K warps, then V warps
             float* prm = reinterpret_cast<float*>(tc_smem + L::kPrmOff);
             if (warp == kSW)
-                load_granules<T, D>(dp, cache, lane, item_lo, item_hi, tc_smem + L::kRawOff, bar_raw, prm, bar_prm);
+                load_granules<T, D>(dp, cache, lane, item_lo, item_hi, sRaw, bar_raw);
             else if (who < kTcUnpackK)
-                unpack_operand<T, D, false>(dp, who, lane, item_lo, item_hi, sK, tc_smem + L::kRawOff, bar_full_k, bar_empty_k, bar_raw);
+                unpack_operand<T, D, false>(dp, who, lane, item_lo, item_hi, sK, tc_smem + L::kRawOff, bar_full_k, bar_empty_k,
+                                             bar_raw, prm, bar_prm);
             else
                 unpack_operand<T, D, true>(dp, who - kTcUnpackK, lane, item_lo, item_hi, sV, tc_smem + L::kRawOff, bar_full_v,
-                                            bar_empty_v, bar_raw);
+                                            bar_empty_v, bar_raw, prm, bar_prm);
         }
     } else if (!kInt4 && warp != kSW + 1) {
         // ---- TMA producers: one warp streams K, one streams V ---------------------------------
@@ -889,7 +870,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
         for (int j = 0; j < n_tiles; ++j, ++t) {
             if (ok) ok = mbar_wait_in<kInt4>(bar_s + 8 * s, ph, p.wait_ns);
             if constexpr (kInt4) {
-                if (ok) ok = mbar_wait_in<kInt4>(bar_prm + 8 * (t % L::kPrmRing), (t / L::kPrmRing) & 1, p.wait_ns);     // (long done)
+                if (ok) ok = mbar_wait_in<kInt4>(bar_prm + 8 * (t & 3), (t >> 2) & 1, p.wait_ns);     // long done: before the K tile was full
             }
             tc_fence_after();
             if (j == n_tiles - 1 && item + 1 < item_hi) {
@@ -919,7 +900,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
             float sc[CH];
             tmem_ld_f<CH>(lane_addr + s * kTcTile + half * CH, sc);
             if constexpr (kInt4) {
-                const float* prm = reinterpret_cast<const float*>(tc_smem + L::kPrmOff) + (t % L::kPrmRing) * 256 + half * CH;
+                const float* prm = reinterpret_cast<const float*>(tc_smem + L::kPrmOff) + (t & 3) * 256 + half * CH;
                 const uint64_t qq = pack_f32x2(q_sum, q_sum);
 #pragma unroll
                 for (int i = 0; i < CH; i += 4) {       // (the same address in every lane: broadcasts)
