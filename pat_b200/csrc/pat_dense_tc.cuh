@@ -48,7 +48,7 @@ constexpr int kTcTile = 128;                // tokens per tile
 constexpr int kTcRing = 3;                  // depth of the K, V and S rings
 constexpr int kTcSoftmaxWarps = 8;
 constexpr int kTcThreads = (kTcSoftmaxWarps + 3) * 32;
-// 4-bit cache: warp 8 requests the raw tiles, warps 10-15 unpack.  Sixteen warps start with 128 registers a thread (the register file);
+// 4-bit cache: warp 8 requests the raw tiles, warps 10 to 15 unpack.  Sixteen warps start with 128 registers a thread (the register file);
 // the unpacking warpgroups hand 40 of them each to the softmax warpgroups.
 constexpr int kTcUnpackK = 2, kTcUnpackV = 4;       // warps per operand: V takes twice the arithmetic
 constexpr int kTcUnpackWarps = kTcUnpackK + kTcUnpackV;
@@ -575,7 +575,9 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
     if constexpr (kInt4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcUnpackRegs));
     if (kInt4 && warp != kSW + 1) {
         if constexpr (kInt4) {
-            const int who = warp - kSW - 2;                         // K warps, then V warps
+            // K on warps 12 and 13, which share their quarters of the SM with the loading warp and the MMA warp; V, the
+            // heavier part, in pairs on the other two quarters (the other way round a tile took 5 % longer)
+            const int who = warp < 12 ? warp - 8 : warp < 14 ? warp - 12 : warp - 10;      // 0, 1: K; 2 .. 5: V
             float* prm = reinterpret_cast<float*>(tc_smem + L::kPrmOff);
             if (warp == kSW)
                 load_granules<T, D>(dp, cache, lane, item_lo, item_hi, sRaw, bar_raw);
