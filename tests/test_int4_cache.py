@@ -426,6 +426,38 @@ def test_scores_of_any_size(dtype, native_lib):
 
 
 @gpu
+@pytest.mark.parametrize("dim,tokens", [(128, 8192), (64, 5000)])
+def test_long_unit_keeps_its_precision(dim, tokens, monkeypatch, native_lib):
+    """A unit as long as a whole context, all weights equal: the mean of many values of either sign.
+
+    q = 0 makes every weight 1 and P' = s exactly (the model's type is fp16), so that only fp32 sums and the output's
+    rounding are left.  A tensor-core sum of 16 products and its accumulator loses at most 2^-23 of the sum of
+    their magnitudes: products up to 79 s, at most 128 tokens' of them before the constant in them is taken out, beside
+    the running sum, once a tile.  That is tiles * 2^-23 * (9 * 16 * 79 s + the largest running sum) over the tokens;
+    the taking out, twice 2^-24 of as much once in 8 tiles, is within the factor 9 (the sum grows to 8 tiles' only at a
+    window's end).  The middles lo + 7.5 s are summed in fp32 per lane: 2^-24 of the largest running sum per token."""
+    import pat_b200._prefix_attn as P
+    cfg = P.int4_config()
+    cfg.num_sms, cfg.items_per_sm, cfg.chunk_tokens_min, cfg.chunk_tokens_max = 1, 1, 1 << 16, 1 << 16
+    monkeypatch.setattr(P, "int4_config", lambda: cfg)
+    pages = -(-tokens // 16)
+    key, value = _rows(pages * 16, 1, dim, FP16, 12)
+    cache = torch.zeros(int4_cache_shape(pages, 16, 1, dim), dtype=torch.uint8, device=DEV)
+    reshape_and_cache_int4(key.to(DEV), value.to(DEV), cache, torch.arange(pages * 16, device=DEV))
+    tree = _tree([tokens], [list(range(pages))], 16, 8, 1)
+    q = torch.zeros(1, 1, 8, dim, dtype=FP16, device=DEV)
+    out = torch.empty_like(q)
+    prefix_attn_with_int4_kvcache(q, cache, tree, 0.1, out)
+    v = I.read(cache.cpu(), dim, FP16)[1].reshape(-1, dim)[:tokens].double()
+    want = v.mean(0)
+    s = float((v.amax(-1) - v.amin(-1)).max() / 15)
+    run = float(v.cumsum(0).abs().max() + (v.amax(-1) + v.amin(-1)).cumsum(0).abs().max())
+    tol = want.abs() * 2.0 ** -11 + 2.0 ** -23 / 16 * (9 * 16 * 79 * s + run) + 2.0 ** -24 * run
+    err = (out[0, 0].double().cpu() - want).abs()
+    assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the bound"
+
+
+@gpu
 @pytest.mark.parametrize("T", [1, 4])
 def test_what_lies_behind_a_sequence_is_not_read(T, native_lib):
     """NaN scales behind the last token of every page list (and in pages of nobody) change nothing; with
