@@ -119,7 +119,8 @@ def beam_select(logits, scores, num_out, finished=None, pad_token=0):
                 if finished is not None and bool(finished[b, k]):
                     row[pad_token] = sc
                 elif not bool((torch.isnan(x) | (x == float("inf"))).any()) and bool((x > float("-inf")).any()):
-                    row = sc + (x - torch.logsumexp(x, 0))
+                    below = x - x.max()             # (first: 64 bits do not hold 3e38 + log n)
+                    row = sc + (below - torch.logsumexp(below, 0))
             rows.append(row)
         flat = torch.cat(rows).numpy()
         order = np.lexsort((np.arange(flat.size), -flat))[:num_out]

@@ -7,6 +7,7 @@ host bookkeeping like the radix tree, since the plan of a step is made on the ho
 from __future__ import annotations
 
 import struct
+from operator import index as index_of
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -32,6 +33,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int, finish
     beyond the first of a search that starts), or whose logits hold a NaN or +inf or nothing but -inf, takes no
     part; where an entry has fewer finite values than ``num_out``, -inf entries follow, lowest beam and
     token first.  ``num_out`` <= 128, ``beams`` <= 512, ``vocab`` <= 2^24."""
+    num_out, pad_token = index_of(num_out), index_of(pad_token)
     sig = (logits.dtype, logits.shape, logits.stride(), logits.get_device(), scores.dtype, scores.shape, scores.stride(),
            scores.get_device(), num_out, pad_token)
     if finished is not None:
@@ -135,6 +137,8 @@ class PagePool:
 
     def alloc(self, count: int) -> List[int]:
         """``count`` free pages, lowest ids first."""
+        if count < 0:
+            raise ValueError("count must not be negative")
         free = np.flatnonzero(self.uses == 0)[:count]
         if len(free) < count:
             raise RuntimeError(f"the cache is full: {count} pages asked for, {len(free)} free")
@@ -178,6 +182,10 @@ class PagePool:
         few free pages."""
         tables = [list(t) for t in tables]
         parents = [int(p) for p in parents]
+        if len(lens) != len(tables) or any(n < 0 or len(t) * self.page_size < n for t, n in zip(tables, lens)):
+            raise RuntimeError("lens must give every table a length that its pages hold")
+        for t in tables:
+            self._in_use(t)
         for p in parents:
             if not 0 <= p < len(tables):
                 raise RuntimeError("parent outside the batch")
@@ -203,7 +211,7 @@ class PagePool:
 
     def compact(self, tables: Sequence[Sequence[int]]) -> Tuple[List[List[int]], List[Tuple[int, int]]]:
         """Moves the pages in use to the front: with ``n`` pages in use, those beyond page ``n`` go to the free
-        ones before it.  Returns the new tables and the ``(from, to)`` pairs; targets are free pages, so
+        ones before it.  ``tables``: those of all requests.  Returns the new tables and the ``(from, to)`` pairs; targets are free pages, so
         never sources."""
         used = np.flatnonzero(self.uses > 0)
         n = len(used)

@@ -208,10 +208,12 @@ def copy_pages(caches: Union[torch.Tensor, Sequence[torch.Tensor]], mapping) -> 
     caches = [caches] if isinstance(caches, torch.Tensor) else caches
     on_device = isinstance(mapping, torch.Tensor) and mapping.is_cuda
     if not on_device:
-        mapping = torch.as_tensor(mapping, dtype=torch.int64)
+        mapping = torch.as_tensor(mapping)
         if mapping.numel() == 0:
             mapping = mapping.reshape(0, 2)
-        mapping = mapping.contiguous()
+        elif mapping.is_floating_point() or mapping.is_complex() or mapping.dtype == torch.bool:
+            raise RuntimeError("mapping must hold integers")
+        mapping = mapping.to(torch.int64).contiguous()
     if mapping.dim() != 2 or mapping.shape[1] != 2:
         raise RuntimeError("mapping must be [n, 2]: pairs (from, to)")
     if on_device and (mapping.dtype != torch.int64 or not mapping.is_contiguous()):

@@ -48,7 +48,7 @@ struct BeamParams {
     float* list_x;                 // [rows][chunks][num_out]
     int32_t* list_v;
     int32_t* list_n;               // [rows][chunks]
-    float* chunk_ref;              // reference of the sum, in powers of two; +inf: NaN or +inf seen, -inf: nothing but -inf
+    float* chunk_ref;              // largest logit, which the sum is relative to; +inf: NaN or +inf seen, -inf: nothing but -inf
     double* chunk_sum;
     int batch, beams, vocab, num_out, chunks, chunk_len, pad_token;
 };
@@ -58,12 +58,13 @@ template <> __device__ __forceinline__ float to_float<float>(float v) { return v
 template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// 2^(x log2(e) - ref), log2(e) in two parts.  The reference is whatever float lies near the largest x log2(e), and the
-// sums are exact about it: nothing but the rounding of each argument is lost.
+// e^d of a difference d <= 0, log2(e) in two parts.  The difference to the maximum is rounded, not the two logits times
+// log2(e): logits of any finite size keep their sum (a difference d's rounding weighs e^d d 2^-24), and -3e38 beside
+// 3e38 becomes -inf.
 constexpr float kLog2eHi = 1.44269502162933349609375f, kLog2eLo = 1.925963033500011e-08f;
-__device__ __forceinline__ float exp2_about(float x, float ref) {
+__device__ __forceinline__ float exp_below(float d) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(x, kLog2eHi, fmaf(x, kLog2eLo, -ref))));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, kLog2eHi, d * kLog2eLo)));
     return y;
 }
 __device__ __forceinline__ float max_or_nan(float a, float b) {
@@ -174,12 +175,11 @@ template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 5
         return;
     }
 
-    const float ref = m * kLog2eHi;
     float sum = 0.f;
 #pragma unroll
     for (int gi = 0; gi < kGroups; ++gi) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += exp2_about(x[gi * 8 + i], ref);
+        for (int i = 0; i < 8; ++i) sum += exp_below(x[gi * 8 + i] - m);
         if (group[gi] >= edge && group[gi] > -INFINITY) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -201,7 +201,7 @@ template <typename T, int kGroups> __global__ void __launch_bounds__(kThreads, 5
     if (tid == 0) {
         double z = 0.0;
         for (int w = 0; w < kWarps; ++w) z += s_sum[w];
-        p.chunk_ref[slot] = ref;
+        p.chunk_ref[slot] = m;
         p.chunk_sum[slot] = z;
         p.list_n[slot] = found < p.num_out ? found : p.num_out;
     }
@@ -253,7 +253,8 @@ __device__ __forceinline__ bool before(double xa, int64_t ia, double xb, int64_t
 __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p) {
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    __shared__ double s_shift[kMaxBeams];          // score - log-sum; NaN: the beam takes no part
+    __shared__ double s_shift[kMaxBeams];          // score - log(sum); NaN: the beam takes no part
+    __shared__ float s_top[kMaxBeams];             // largest logit
     __shared__ float s_edge[kWarps];
     __shared__ double s_val[kListCap];
     __shared__ int64_t s_idx[kListCap];
@@ -263,12 +264,12 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p)
     s_used[tid] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // log-sum of every beam: ln 2 * (ref + log2 sum)
+    // log-sum of every beam: its largest logit + log(sum)
     for (int k = warp; k < p.beams; k += kWarps) {
         double shift = NAN;
+        float m = -INFINITY;
         if (beam_is_live(p, b, k)) {
             const size_t slot = (static_cast<size_t>(b) * p.beams + k) * p.chunks;
-            float m = -INFINITY;
             for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.chunk_ref[slot + c]);
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
@@ -276,14 +277,14 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p)
                 double z = 0.0;
                 for (int c = lane; c < p.chunks; c += 32) {
                     const float ref = p.chunk_ref[slot + c];
-                    if (ref > -INFINITY) z += p.chunk_sum[slot + c] * exp2(static_cast<double>(ref) - static_cast<double>(m));
+                    if (ref > -INFINITY) z += p.chunk_sum[slot + c] * exp(static_cast<double>(ref) - static_cast<double>(m));
                 }
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) z += __shfl_xor_sync(kFull, z, d);
-                shift = static_cast<double>(p.scores[b * p.score_stride + k]) - 0.693147180559945309417 * (static_cast<double>(m) + log2(z));
+                shift = static_cast<double>(p.scores[b * p.score_stride + k]) - log(z);
             }
         }
-        if (lane == 0) s_shift[k] = shift;
+        if (lane == 0) { s_shift[k] = shift; s_top[k] = m; }
     }
     __syncthreads();
 
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const BeamParams p)
             const float x = my_x[list * p.num_out + pos];      // (may hold anything behind the list's end)
             const int n = p.list_n[static_cast<size_t>(b) * lists + list];
             const double shift = s_shift[list / p.chunks];
-            return pos < n && shift == shift ? shift + static_cast<double>(x) : -INFINITY;
+            return pos < n && shift == shift ? shift + (static_cast<double>(x) - static_cast<double>(s_top[list / p.chunks])) : -INFINITY;
         }
         const int k = j - (lists << shift_out);
         const float score = p.scores[b * p.score_stride + k];

@@ -74,6 +74,18 @@ def test_fork_that_does_not_fit_changes_nothing():
         pool.fork(tables, lens, [1])
 
 
+def test_pool_refuses_what_does_not_fit_together():
+    pool = PagePool(6, 4)
+    tables = [pool.alloc(2)]
+    before = pool.uses.copy()
+    for bad in [(tables, [9], [0]), (tables, [-1], [0]), (tables, [5, 5], [0]), ([[0, 4]], [5], [0]), ([[0, 7]], [5], [0])]:
+        with pytest.raises(RuntimeError):
+            pool.fork(*bad)
+    with pytest.raises(ValueError):
+        pool.alloc(-1)
+    assert np.array_equal(before, pool.uses)
+
+
 @pytest.mark.parametrize("seed", range(5))
 def test_random_searches_keep_every_token(seed):
     """A model of the cache on the host: after forks, copies, appends and compactions every request still
@@ -126,6 +138,11 @@ def test_host_tensors_and_bad_mappings_are_refused(native_lib):
         copy_pages(torch.zeros(4, 16), [0, 1, 2])
     with pytest.raises(RuntimeError, match="CUDA"):
         beam_select(torch.zeros(1, 2, 8), torch.zeros(1, 2), 2)
+    for bad in ([(0.5, 1.0)], torch.tensor([[0.0, 1.0]]), [(True, False)]):
+        with pytest.raises(RuntimeError, match="integers"):
+            copy_pages(torch.zeros(4, 16), bad)
+    with pytest.raises(TypeError):
+        beam_select(torch.zeros(1, 2, 8), torch.zeros(1, 2), 2.5)
     copy_pages([], [(0, 1)])
 
 
@@ -290,6 +307,19 @@ def test_first_step_and_empty_entries(native_lib):
     logits[2, 0, 3:] = float("-inf")                   # three finite values, eight asked for
     logits[2, 0, 1] = float("-inf")
     _check_beam(logits, scores, 8)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_of_any_finite_size(dtype, native_lib):
+    logits, scores = _logits(4, 3, 9000, dtype, 6)
+    logits[0, 1, 8500] = 3e38                           # all of its beam's probability
+    logits[1, 2] = -3e38                                # its beam's tokens are equal
+    logits[2, :, 4:] = -3e38                            # four tokens a beam
+    logits[3, 0, 5] = -2.5e38
+    logits[3, 1, 7], logits[3, 1, 8] = 1.5e38, -1.5e38
+    logits[3, 2] += 1e6
+    _check_beam(logits, scores, 16)
 
 
 @gpu
