@@ -921,17 +921,16 @@ def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree,
 
     ``kv_cache``: uint8 ``[pages, kv_heads, page_size / 16, tile bytes]`` as ``cache_ops.int4_cache_shape``
     gives it, filled by ``cache_ops.reshape_and_cache_int4`` with rows of ``q``'s dtype; page and head strides are
-    free.  ``tree``: a ``PrefixTreeCPP`` (or an ``AsyncTree`` holding one) whose plan was sent with
-    ``kernel_info.to_gpu(device, kv_cache_dtype="int4")``.  ``q``, ``out``, ``softmax_scale`` and ``lse_out`` are
+    free.  ``tree``: a ``PrefixTreeCPP`` (or an ``AsyncTree`` made with ``kv_cache_dtype="int4"``) whose plan was
+    sent with ``kernel_info.to_gpu(device, kv_cache_dtype="int4")``.  ``q``, ``out``, ``softmax_scale`` and ``lse_out`` are
     those of ``prefix_attn_with_kvcache``, several query tokens per request included.  A request (or
     position) that sees no token gets zeros, and -inf in ``lse_out``.
 
     The products run on the exact codes; scales, offsets, softmax and sums are fp32, and the
     probabilities are rounded to ``q``'s dtype for the second product as in the 16-bit op."""
-    if not isinstance(tree, PrefixTreeCPP):
-        tree = getattr(tree, "tree", None)      # an AsyncTree hands over its built tree
-        _check(isinstance(tree, PrefixTreeCPP), "tree must be a PrefixTreeCPP")
-    index = q.get_device()
+    tree = getattr(tree, "tree", tree)          # an AsyncTree hands over its built tree
+    _check(isinstance(tree, PrefixTreeCPP), "tree must be a PrefixTreeCPP")
+    index, softmax_scale = q.get_device(), float(softmax_scale)
     # What depends on types, shapes, strides and devices alone is checked once per work list.
     sig = (q.dtype, q.shape, q.stride(), index, kv_cache.dtype, kv_cache.shape, kv_cache.stride(), kv_cache.get_device(),
            out.dtype, out.shape, out.stride(), out.get_device(), softmax_scale, _flags, _wait_limit_us, _config_epoch)

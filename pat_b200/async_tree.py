@@ -20,7 +20,8 @@ from ._prefix_attn import PrefixTreeCPP
 
 class AsyncTree(PrefixTreeCPP):
     def __init__(self, block_size: int, seq_lens: Union[List[int], torch.Tensor], table: torch.Tensor,
-                 MNWs: Union[None, List[List[int]]], HRatio: int, kvHead: int, device: torch.device):
+                 MNWs: Union[None, List[List[int]]], HRatio: int, kvHead: int, device: torch.device,
+                 kv_cache_dtype: str = "auto"):
         super().__init__(block_size)
         self._tree: Optional[PrefixTreeCPP] = None
         self._init_time = time.time()
@@ -29,7 +30,7 @@ class AsyncTree(PrefixTreeCPP):
             built = PrefixTreeCPP(block_size)
             built.build_radix_tree(seq_lens, table)
             built.pack_schedule(MNWs=MNWs, HRatio=HRatio, kvHead=kvHead)
-            built.kernel_info.to_gpu(device)
+            built.kernel_info.to_gpu(device, kv_cache_dtype)
             return built
 
         self._pool = ThreadPoolExecutor(max_workers=1)

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import int4_oracle as I
-from pat_b200 import DecodePlanner, PrefixTreeCPP, prefix_attn_with_int4_kvcache
+from pat_b200 import AsyncTree, DecodePlanner, PrefixTreeCPP, prefix_attn_with_int4_kvcache
 from pat_b200 import _native as N
 from pat_b200.cache_ops import (gather_cache_int4, int4_cache_shape, int4_tile_bytes, reshape_and_cache_flash,
                                 reshape_and_cache_int4)
@@ -118,6 +118,13 @@ def test_attention_refuses_bad_arguments(field, value, code, native_lib):
     a = _decode_args(native_lib)
     setattr(a, field, value)
     assert native_lib.pat_b200_decode_int4(C.byref(a), None) == code
+
+
+def test_async_tree_makes_the_plan_of_its_cache(native_lib):
+    at = AsyncTree(16, [5, 20], torch.tensor([[0, 0], [1, 2]], dtype=torch.int32), None, 4, 2, torch.device("cpu"), kv_cache_dtype="int4")
+    assert isinstance(at.tree, PrefixTreeCPP)
+    with pytest.raises(RuntimeError, match="fp8"):
+        AsyncTree(16, [5], torch.tensor([[0]], dtype=torch.int32), None, 4, 2, torch.device("cpu"), kv_cache_dtype="fp8").tree
 
 
 # ------------------------------------------------------------------------------------------ GPU
@@ -642,6 +649,21 @@ def test_append_then_attend(native_lib):
     torch.cuda.synchronize()
     # both within 2e-2 of the same exact result; the 16-bit rows are rounded values of the codes
     assert float((out.float() - wide.float()).abs().max()) <= 2e-2
+
+
+@gpu
+def test_attention_with_an_async_tree(native_lib):
+    lens, tables, pages = _batch("shared", 16, 4)
+    cache = _fill(pages, 16, 2, 64, BF16, 4)
+    table = torch.zeros(len(lens), max(len(t) for t in tables), dtype=torch.int32)
+    for i, t in enumerate(tables):
+        table[i, :len(t)] = torch.tensor(t, dtype=torch.int32)
+    at = AsyncTree(16, lens, table, None, 4, 2, torch.device(DEV), kv_cache_dtype="int4")
+    q = torch.randn(len(lens), 1, 8, 64, dtype=BF16, device=DEV)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    prefix_attn_with_int4_kvcache(q, cache, at, 0.125, a)
+    prefix_attn_with_int4_kvcache(q, cache, _tree(lens, tables, 16, 4, 2), 0.125, b)
+    assert torch.equal(a, b)
 
 
 @gpu
