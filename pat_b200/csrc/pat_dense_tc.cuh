@@ -35,7 +35,7 @@
 // cancels in O / l), so the O accumulator in TMEM is rescaled rarely.
 // Every mbarrier wait is bounded.  A wait that gives up records a code in the status word; the
 // role that gave up issues nothing more (no TMA request, no MMA), waits briefly for what it had
-// in flight, the other roles' waits then run out too, and all eleven warps meet at one barrier
+// in flight, the other roles' waits then run out too, and all the warps meet at one barrier
 // before the CTA frees its TMEM and returns.
 #pragma once
 
@@ -61,6 +61,10 @@ constexpr float kTcLazyLog2 = 8.0f;
 
 // kInt4: the cache holds 4-bit codes (pat_int4.cuh).  Raw tiles arrive in granules of 64 tokens (half a tile), in a
 // ring of their own that covers the way from memory; the unpacked tiles then need two slots each.
+//
+// 240 items of 128 rows over 229376 tokens x 8 heads of 128 elements (long shared prefixes): 191 us = 1.9 us per tile of 128 x
+// 128, 630 TFLOP/s in the products; the 16-bit kernel takes 1.2 us per tile.  Tensor pipe 30 % busy, DRAM 8 %, issue slots
+// 60 %: the instructions of unpacking and of the softmax, in one SM's four issue ports, are what it waits for.
 template <int D, bool kInt4> struct TcSmem {
     static constexpr int kBoxes = D / 64;
     static constexpr int kKvRing = kInt4 ? 2 : kTcRing;

