@@ -927,8 +927,8 @@ def prefix_attn_with_int4_kvcache(q: torch.Tensor, kv_cache: torch.Tensor, tree,
     position) that sees no token gets zeros, and -inf in ``lse_out``.
 
     Scales, offsets, softmax and sums are fp32, scores those of the exact codes.  For the second product the
-    probabilities are rounded to ``q``'s dtype (times the scale to fp16 where few rows share a segment), as in
-    the 16-bit op, and where many rows share one (33 and more) so are the values ``lo + s * c``."""
+    probabilities, times the values' scales, are rounded to 16 bits as in the 16-bit op (to fp16 where few rows
+    share a segment, to ``q``'s dtype where 33 and more do); the codes of V are exact."""
     tree = getattr(tree, "tree", tree)          # an AsyncTree hands over its built tree
     _check(isinstance(tree, PrefixTreeCPP), "tree must be a PrefixTreeCPP")
     index, softmax_scale = q.get_device(), float(softmax_scale)

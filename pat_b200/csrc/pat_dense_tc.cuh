@@ -62,13 +62,13 @@ constexpr float kTcLazyLog2 = 8.0f;
 // kInt4: the cache holds 4-bit codes (pat_int4.cuh).  Raw tiles arrive in granules of 64 tokens (half a tile), in a
 // ring of their own that covers the way from memory; the unpacked tiles then need two slots each.
 //
-// 240 items of 128 rows over 229376 tokens x 8 heads of 128 elements (long shared prefixes): 191 us = 1.9 us per tile of 128 x
-// 128, 630 TFLOP/s in the products; the 16-bit kernel takes 1.2 us per tile.  Tensor pipe 30 % busy, DRAM 8 %, issue slots
-// 60 %: the instructions of unpacking and of the softmax, in one SM's four issue ports, are what it waits for.
+// 240 items of 128 rows over 229376 tokens x 8 heads of 128 elements (long shared prefixes): 214 us = 2.1 us per tile of 128 x
+// 128, 560 TFLOP/s in the products; the 16-bit kernel takes 1.2 us per tile.  Tensor pipe under 30 % busy, DRAM 8 %, issue
+// slots about 60 %: the instructions of unpacking and of the softmax, in one SM's four issue ports, are what it waits for.
 template <int D, bool kInt4> struct TcSmem {
     static constexpr int kBoxes = D / 64;
     static constexpr int kKvRing = kInt4 ? 2 : kTcRing;
-    static constexpr int kPrmRing = 4, kRawRing = 7;
+    static constexpr int kPrmRing = 4, kRawRing = 6;
     static constexpr int kRawBytes = 4 * Int4Tile<D>::kBytes;
     static constexpr int kQBytes = kBoxes * 128 * 128;          // [box][128 rows][128 B]
     static constexpr int kKBytes = kBoxes * kTcTile * 128;      // [box][128 tokens][128 B]
@@ -76,10 +76,11 @@ template <int D, bool kInt4> struct TcSmem {
     static constexpr int kKOff = kQOff + kQBytes;               // K ring
     static constexpr int kVOff = kKOff + kKvRing * kKBytes;     // V ring
     static constexpr int kRawOff = kVOff + kKvRing * kKBytes;
-    static constexpr int kBarOff = kRawOff + (kInt4 ? kRawRing * kRawBytes : 0);    // 43 mbarriers (kInt4: 61) + tmem base word + flag
+    static constexpr int kBarOff = kRawOff + (kInt4 ? kRawRing * kRawBytes : 0);    // 43 mbarriers (kInt4: 59) + tmem base word + flag
     static constexpr int kXchOff = kBarOff + 512;               // float[2][2][128]: row maxima / sums of the two column halves
-    static constexpr int kPrmOff = kXchOff + 2048;              // kInt4: float[ring][2][128], factor and addend of every token's scores
-    static constexpr int kRequest = kPrmOff + (kInt4 ? kPrmRing * 1024 : 0);
+    static constexpr int kPrmOff = kXchOff + 2048;              // kInt4: float[ring][4][128], what softmax warps need of every token (below)
+    static constexpr int kPrmFloats = 4 * 128;
+    static constexpr int kRequest = kPrmOff + (kInt4 ? kPrmRing * kPrmFloats * 4 : 0);
 };
 
 // ---- tcgen05 wrappers ------------------------------------------------------------
@@ -252,8 +253,11 @@ struct DenseTcParams {
 //
 // K: the codes go to the tensor cores as they are (16 + c, exact), and the softmax warps turn a product into a
 // score with the token's scale and offset in fp32:  x = (s (q . (16 + c)) + (lo - 16 s) sum(q)) * scale * log2 e.
-// (Rounded K values would put 2^-9 of noise into every bf16 score and through it into the LSE.)  V: values in
-// the model's type, v = lo + s c in one fma of the exact code, rounded once - half a step, like P beside it.
+// (Rounded K values would put 2^-9 of noise into every bf16 score and through it into the LSE.)  V is exact as well:
+// with s = 2^e f, 1 <= f < 2, the operand is (c - 7.5) 2^e, the softmax warps write P' = p f - the one rounding - and
+// add up p (lo + 7.5 s) in fp32.  (Values lo + s c rounded to the model's type are 10 % faster on long shared prefixes, 191 us against 214, and 2 to 7 % on
+// trees, but the output's error is then 1.7 times that of its own rounding instead of 1.4 times.)  A
+// subnormal scale takes the smallest normal power of two and f below 1.
 // A token past the item's end becomes zeros.  One whose V row is NaN gets zeros for V and NaN scores: whoever sees
 // it returns NaN, and for rows that must not see it (kLimits) 0 * V stays 0.
 //
@@ -264,17 +268,19 @@ struct DenseTcParams {
 template <typename T> struct Pack2;
 template <> struct Pack2<__nv_bfloat16> {
     using V = __nv_bfloat162;
-    static constexpr uint32_t kExp = 0x7f80u;
+    static constexpr uint32_t kExp = 0x7f80u, kLeast = 0x0080u;      // exponent bits, smallest normal number
+    static constexpr uint32_t kMiddle = 0x41BC41BCu;                // (23.5, 23.5)
 };
 template <> struct Pack2<__half> {
     using V = __half2;
-    static constexpr uint32_t kExp = 0x7c00u;
+    static constexpr uint32_t kExp = 0x7c00u, kLeast = 0x0400u;
+    static constexpr uint32_t kMiddle = 0x4DE04DE0u;
 };
-template <typename T> __device__ __forceinline__ uint32_t code_pair_value(uint32_t sixteen_plus_c, uint32_t ss, uint32_t ll) {
+template <typename T> __device__ __forceinline__ uint32_t code_pair_value(uint32_t sixteen_plus_c, uint32_t power) {
     using V = typename Pack2<T>::V;
-    const uint32_t k16 = Int4Elt<T>::kSixteen;
-    const V c = __hsub2(*reinterpret_cast<const V*>(&sixteen_plus_c), *reinterpret_cast<const V*>(&k16));
-    const V v = __hfma2(c, *reinterpret_cast<const V*>(&ss), *reinterpret_cast<const V*>(&ll));
+    const uint32_t middle = Pack2<T>::kMiddle;
+    const V c = __hsub2(*reinterpret_cast<const V*>(&sixteen_plus_c), *reinterpret_cast<const V*>(&middle));
+    const V v = __hmul2(c, *reinterpret_cast<const V*>(&power));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 // 8 codes of one word (nibble j of the low half: element 2j, of the high half: 2j + 1) -> 16 bytes at `dst`
@@ -284,16 +290,20 @@ template <typename T> __device__ __forceinline__ void store_codes(uint32_t dst, 
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(E::template pair<0>(word)),
                  "r"(E::template pair<1>(word)), "r"(E::template pair<2>(word)), "r"(E::template pair<3>(word)));
 }
-template <typename T> __device__ __forceinline__ void store_values(uint32_t dst, uint32_t word, uint32_t ss, uint32_t ll) {
+template <typename T> __device__ __forceinline__ void store_values(uint32_t dst, uint32_t word, uint32_t power) {
     using E = Int4Elt<T>;
-    const uint32_t a = code_pair_value<T>(E::template pair<0>(word), ss, ll), b = code_pair_value<T>(E::template pair<1>(word), ss, ll);
-    const uint32_t c = code_pair_value<T>(E::template pair<2>(word), ss, ll), d = code_pair_value<T>(E::template pair<3>(word), ss, ll);
+    const uint32_t a = code_pair_value<T>(E::template pair<0>(word), power), b = code_pair_value<T>(E::template pair<1>(word), power);
+    const uint32_t c = code_pair_value<T>(E::template pair<2>(word), power), d = code_pair_value<T>(E::template pair<3>(word), power);
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d));
 }
-// scale and offset of a token, each doubled to a pair
-__device__ __forceinline__ void split_params(uint32_t prm, uint32_t& ss, uint32_t& ll) {
-    ss = __byte_perm(prm, prm, 0x1010);
-    ll = __byte_perm(prm, prm, 0x3232);
+// the power of two of a token's scale, twice
+template <typename T> __device__ __forceinline__ uint32_t power_pair(uint32_t prm) {
+    return max(prm & Pack2<T>::kExp, Pack2<T>::kLeast) * 0x10001u;
+}
+// its other factor
+template <typename T> __device__ __forceinline__ float scale_factor(float scale) {
+    const uint32_t least = Int4Elt<T>::kIsHalf ? 113u << 23 : 1u << 23;
+    return scale * __uint_as_float((254u << 23) - max(__float_as_uint(scale) & 0x7f800000u, least));
 }
 template <typename T> __device__ __forceinline__ bool params_are_finite(uint32_t prm) {
     constexpr uint32_t e = Pack2<T>::kExp;
@@ -417,15 +427,24 @@ __device__ __forceinline__ void unpack_operand(const DenseTcParams& dp, int who,
                     static_assert(kTcUnpackK == 2, "32 of a granule's tokens per warp");
                     const int tok = lane + 32 * who, row = half * 64 + tok;
                     const unsigned char* src = rt + (tok >> 4) * I::kBytes + (tok & 15) * 4;
-                    float factor = 0.f, addend = 0.f;
+                    float factor = 0.f, addend = 0.f, v_factor = 0.f, v_middle = 0.f;
                     if (row < valid) {
                         const float2 kp = Int4Elt<T>::unpack(*reinterpret_cast<const uint32_t*>(src + I::kKPrm));
+                        const uint32_t v_prm = *reinterpret_cast<const uint32_t*>(src + I::kVPrm);
+                        const float2 vp = Int4Elt<T>::unpack(v_prm);
                         factor = kp.x * p.scale_log2;
-                        addend = params_are_finite<T>(*reinterpret_cast<const uint32_t*>(src + I::kVPrm))
-                                     ? (kp.y - 16.f * kp.x) * p.scale_log2 : NAN;
+                        addend = NAN;
+                        if (params_are_finite<T>(v_prm)) {
+                            addend = (kp.y - 16.f * kp.x) * p.scale_log2;
+                            v_factor = scale_factor<T>(vp.x);
+                            v_middle = fmaf(7.5f, vp.x, vp.y);
+                        }
                     }
-                    prm[(t & 3) * 256 + row] = factor;
-                    prm[(t & 3) * 256 + 128 + row] = addend;
+                    float* to = prm + (t & 3) * L::kPrmFloats + row;
+                    to[0] = factor;
+                    to[128] = addend;
+                    to[256] = v_factor;
+                    to[384] = v_middle;
                 }
 #pragma unroll 1
                 for (int u = who; u < 4; u += kGroup) {         // 16 tokens, as two units whose arithmetic interleaves
@@ -461,15 +480,15 @@ __device__ __forceinline__ void unpack_operand(const DenseTcParams& dp, int who,
                             for (int e = 0; e < 2; ++e) {
                                 const uint32_t vp = e == 0 ? prm2[h].x : prm2[h].y;
                                 const bool keep = static_cast<int>(row0) + 2 * c + 8 * h + e < valid && params_are_finite<T>(vp);
-                                uint32_t ss, ll, y[kWords / 2];      // words of 8 consecutive dims of this token
-                                split_params(keep ? vp : 0u, ss, ll);
+                                const uint32_t power = keep ? power_pair<T>(vp) : 0u;
+                                uint32_t y[kWords / 2];              // words of 8 consecutive dims of this token
 #pragma unroll
                                 for (int i = 0; i < kWords / 2; ++i)
                                     y[i] = __byte_perm(w[h][2 * i], w[h][2 * i + 1], e == 0 ? 0x5410 : 0x7632);
 #pragma unroll
                                 for (int i = 0; i < kWords / 2; ++i)
                                     store_values<T>(dst + h * 1024 + place[e * (kWords / 2) + i],
-                                                    D == 128 && (g & 1) ? y[i ^ 1] : y[i], ss, ll);
+                                                    D == 128 && (g & 1) ? y[i ^ 1] : y[i], power);
                             }
                     }
                 }
@@ -538,7 +557,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
                    bar_ofree = bars + 56 * R + 8, bar_drain = bars + 56 * R + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tc_smem + L::kBarOff + 56 * R + 24);
     volatile int* poisoned = reinterpret_cast<volatile int*>(tc_smem + L::kBarOff + 56 * R + 32);
-    const uint32_t bar_prm = bars + 56 * R + 40, bar_raw = bar_prm + 32;        // kInt4: [4]; full [7], empty [7]
+    const uint32_t bar_prm = bars + 56 * R + 40, bar_raw = bar_prm + 32;        // kInt4: [4]; full [6], empty [6]
     float* xch = reinterpret_cast<float*>(tc_smem + L::kXchOff);      // [2][2][128]
 
     // If an earlier CTA of this call already gave up on a wait, do not start (uniform decision).
@@ -873,6 +892,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
         }
 
         float m_used = -INFINITY, l = 0.f;
+        uint64_t mid = 0;                   // kInt4: sums of p (lo + 7.5 s) over the even and the odd tokens
         for (int j = 0; j < n_tiles; ++j, ++t) {
             if (ok) ok = mbar_wait_in<kInt4>(bar_s + 8 * s, ph, p.wait_ns);
             if constexpr (kInt4) {
@@ -906,7 +926,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
             float sc[CH];
             tmem_ld_f<CH>(lane_addr + s * kTcTile + half * CH, sc);
             if constexpr (kInt4) {
-                const float* prm = reinterpret_cast<const float*>(tc_smem + L::kPrmOff) + (t & 3) * 256 + half * CH;
+                const float* prm = reinterpret_cast<const float*>(tc_smem + L::kPrmOff) + (t & 3) * L::kPrmFloats + half * CH;
                 const uint64_t qq = pack_f32x2(q_sum, q_sum);
 #pragma unroll
                 for (int i = 0; i < CH; i += 4) {       // (the same address in every lane: broadcasts)
@@ -943,6 +963,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
                 ensure_o(t);            // O may only be touched once every earlier P V has completed
                 const float alpha = raise ? fast_exp2((m_used - mx) * c) : 1.f;
                 l *= alpha;
+                if constexpr (kInt4) mid = mul_f32x2(mid, pack_f32x2(alpha, alpha));
                 float ov[OC];
                 tmem_ld_f<OC>(tmem_o, ov);
 #pragma unroll
@@ -953,6 +974,7 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
             const float off = m_used * c;
             float sum0 = 0.f, sum1 = 0.f;
             uint32_t packed[CH / 2];
+            float4 v_factor = make_float4(0.f, 0.f, 0.f, 0.f), v_middle = v_factor;
             // One exponential per score on the special-function unit (16 per clock and SM) and about
             // as many cycles of FMA-pipe work (scale, sum, 16-bit packing) per tile: moving a share of
             // the exponentials to the FMA pipe as a polynomial made the tile slower, not faster.
@@ -962,7 +984,20 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
                 const float p1 = fast_exp2(fmaf(sc[2 * i + 1], c, -off));
                 sum0 += p0;
                 sum1 += p1;
-                packed[i] = Elt<T>::pack(p0, p1);
+                if constexpr (kInt4) {
+                    const float* of = reinterpret_cast<const float*>(tc_smem + L::kPrmOff) + (t & 3) * L::kPrmFloats + 256 + half * CH;
+                    if ((i & 1) == 0) {                 // (the same address in every lane: broadcasts)
+                        v_factor = *reinterpret_cast<const float4*>(of + 2 * i);
+                        v_middle = *reinterpret_cast<const float4*>(of + 128 + 2 * i);
+                    }
+                    const uint64_t pp = pack_f32x2(p0, p1);
+                    float w0, w1;
+                    unpack_f32x2(mul_f32x2(pp, i & 1 ? pack_f32x2(v_factor.z, v_factor.w) : pack_f32x2(v_factor.x, v_factor.y)), w0, w1);
+                    mid = fma_f32x2(pp, i & 1 ? pack_f32x2(v_middle.z, v_middle.w) : pack_f32x2(v_middle.x, v_middle.y), mid);
+                    packed[i] = Elt<T>::pack(w0, w1);
+                } else {
+                    packed[i] = Elt<T>::pack(p0, p1);
+                }
             }
             l += sum0 + sum1;
             // P over the S columns this row has consumed: CH / 2 packed columns per half
@@ -997,8 +1032,15 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
             float* xbuf = xch + (t & 1) * 256;
             pair_sync();                        // partner has read the last tile's maximum
             xbuf[half * 128 + r] = l;
+            float mid0 = 0.f, mid1 = 0.f;
+            if constexpr (kInt4) {              // (the buffer of the last tile's maxima, read by now)
+                unpack_f32x2(mid, mid0, mid1);
+                mid0 += mid1;
+                xch[((t + 1) & 1) * 256 + half * 128 + r] = mid0;
+            }
             pair_sync();
             const float l_row = l + xbuf[(half ^ 1) * 128 + r];
+            if constexpr (kInt4) mid0 += xch[((t + 1) & 1) * 256 + (half ^ 1) * 128 + r];
             pair_sync();                        // both have read before the buffer is reused
             ensure_o(t);
             const bool store = ok && r < rows_valid;
@@ -1012,6 +1054,10 @@ __device__ __forceinline__ void dense_tc_body(const DenseTcParams& dp, const CUt
             const float inv = seen ? 1.f / l_row : 0.f;
             float ov[OC];
             tmem_ld_f<OC>(tmem_o, ov);
+            if constexpr (kInt4) {
+#pragma unroll
+                for (int i = 0; i < OC; ++i) ov[i] += mid0;
+            }
             tc_fence_before();
             mbar_arrive(bar_ofree);             // O may be overwritten by the next item's first P V
             if (store) {

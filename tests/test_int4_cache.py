@@ -324,9 +324,9 @@ def _batch(kind, page, seed):
 def _bounds(k, v, q, scale, dtype, ref):
     """Largest errors of output and LSE.  With u = half a step of the type:
 
-    * Few rows: P' = p s is rounded once (relative u) and multiplies c - 7.5, which moves sum p s (c - 7.5) by
-      at most u times half the spread of a value row.  Many rows: p and v = lo + s c are rounded once each, which
-      moves sum p v by at most 2 u max |v|.  The output is rounded once (u |out|).
+    * P' = p s (or p times s over a power of two) is rounded once (relative u) and multiplies c - 7.5, which moves
+      sum p s (c - 7.5) by at most u times half the spread of a value row, itself at most max |v|.  The output is
+      rounded once (u |out|).  (2 u max |v| would be p and v = lo + s c rounded once each.)
     * A score is an fp32 sum of 2 D products of at most |q| (16 + 15) s (the codes are exact on both paths):
       2 D roundings of 2^-24 of their sum bound it, and a score's error e changes a weight by a factor of
       1 + 2 e, the output by at most 2 e times the spread of the values.
