@@ -79,12 +79,12 @@ def int4_config() -> WorkConfig:
     """Options of the work lists for a 4-bit cache.
 
     A warp of the streaming kernel takes 8 rows, and a unit is a warp's, not a CTA's: smaller chunks, more of
-    them (128 tokens and 16 per SM against the 16-bit path's 256 and 4: small batch 12.6 -> 8.4 us, deep tree even,
-    long contexts even).  Unpacking a tile costs the dense kernel the same for one row as for 128, so it gets
-    segments of 33 rows on (17: small batch 29 us against 13, two-level tree 69 against 61, deep tree 99
-    against 93; 49 and 65 are even), cut for every SM: neither kernel waits for memory long enough to gain
-    from running beside the other (long contexts 740 us on the 16-bit path's share of the SMs, 535 on all of
-    them).  Figures in microseconds per step on a B200."""
+    them (128 tokens and 16 per SM against the 16-bit path's 256 and 4: small batch 15.6 -> 11.9 us, two-level tree
+    68 -> 62.5, long contexts 403 -> 399, deep tree even; 24 per SM: 12.5, 65, 402 and 89).  Unpacking a tile costs the
+    dense kernel the same for one row as for 128, so it gets segments of 33 rows on (17: small batch 27.7 us against
+    11.9, two-level tree 69 against 62.5, deep tree 97 against 90; 65 is even), cut for every SM: neither kernel
+    waits for memory long enough to gain from running beside the other (long contexts 642 us on the 16-bit path's
+    share of the SMs, 399 on all of them; a two-level tree 64 against 62.5, a deep tree 86.5 against 90).  Figures in microseconds per step on a B200."""
     cfg = WorkConfig(**{n: getattr(default_config(), n) for n in WorkConfig.__slots__})
     cfg.stream_rows = cfg.stream_rows or 8
     cfg.items_per_sm = cfg.items_per_sm or 16
